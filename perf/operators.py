@@ -201,7 +201,7 @@ def _scores(case, logits):
     if case["scoring"] == "sigmoid":
         s = 1.0 / (1.0 + torch.exp(-x.double()).float())
     else:
-        e = torch.exp((x - x.amax(1, keepdim=True)).double()).masked_fill(~open_, 0.0)
+        e = torch.exp(x.double() - x.amax(1, keepdim=True).double()).masked_fill(~open_, 0.0)
         s = (e / e.sum(1, keepdim=True).clamp_min(1e-300)).float()
     return s.masked_fill(~open_, 0.0), open_
 
