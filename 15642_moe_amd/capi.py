@@ -13,7 +13,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("lib15642_moe_fp8.so")
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 MOE_OK = 0
 MOE_ERR_INVALID_ARG = 1
@@ -26,6 +26,11 @@ MAX_T = 262143  # include/moe_fp8.h MOE_MAX_T: 32-bit activation offsets in the 
  WS_QUEUE) = range(11)
 WS_NBUF = 11
 FORWARD_EVENTS = 6
+
+# Operators beside the forward: enum moe_dtype, enum moe_scoring and their limits.
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = range(3)
+SCORING = {"sigmoid": 0, "softmax": 1}
+MAX_EXPERTS, MAX_TOP_K, MAX_W4_DIM = 1024, 64, 262144
 
 _c_int, _c_size, _c_float, _c_vp, _c_u64 = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
 
@@ -63,6 +68,27 @@ SIGNATURES = {
     "moe_unpack_router": (_c_int, [_c_vp, _c_vp, _c_vp]),
     "moe_router_workspace_bytes": (_c_size, [_c_int]),
     "moe_router_quant": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_size, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "moe_route_topk": (
+        _c_int,
+        [_c_vp, _c_int, _c_size, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
+         _c_vp, _c_vp, _c_vp],
+    ),
+    "moe_route_topk_backward": (
+        _c_int,
+        [_c_vp, _c_vp, _c_int, _c_size, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_vp, _c_vp],
+    ),
+    "moe_quant_act": (_c_int, [_c_vp, _c_int, _c_size, _c_int, _c_int, _c_vp, _c_vp, _c_vp]),
+    "moe_quantize_w4": (_c_int, [_c_vp, _c_int, _c_size, _c_vp, _c_vp, _c_vp]),
+    "moe_packed_w4_bytes": (_c_size, [_c_int, _c_int]),
+    "moe_pack_w4": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp]),
+    "moe_unpack_w4": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp]),
+    "moe_linear_w4": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    "moe_experts_w4_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "moe_experts_w4": (
+        _c_int,
+        [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size,
+         _c_vp, _c_vp],
+    ),
     "moe_fill_normal_e4m3": (_c_int, [_c_vp, _c_size, _c_u64, _c_u64, _c_vp]),
     "moe_mfma_tiles": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp]),
     "moe_mfma_ceiling": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, _c_vp]),

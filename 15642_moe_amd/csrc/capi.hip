@@ -378,6 +378,200 @@ int moe_router_quant(const void* hidden_bf16, const void* router_packed, int T, 
                     "router_quant_kernel launch");
 }
 
+static int check_dtype(int dtype) {
+  if (dtype < MOE_DTYPE_F32 || dtype > MOE_DTYPE_F16)
+    return fail(MOE_ERR_INVALID_ARG, "dtype must be one of moe_dtype, got %d", dtype);
+  return MOE_OK;
+}
+static size_t dtype_bytes(int dtype) { return dtype == MOE_DTYPE_F32 ? 4 : 2; }
+static int check_element_ptr(const void* p, size_t bytes, const char* name) {
+  if (!p) return fail(MOE_ERR_INVALID_ARG, "%s must not be null", name);
+  if ((uintptr_t)p % bytes) return fail(MOE_ERR_INVALID_ARG, "%s must be aligned to its elements", name);
+  return MOE_OK;
+}
+
+static int check_router(int dtype, int T, int n_experts, int top_k, int scoring) {
+  if (T < 0 || T > MOE_MAX_ROUTE_T)
+    return fail(MOE_ERR_INVALID_ARG, "T must be in [0, %d], got %d", MOE_MAX_ROUTE_T, T);
+  MOE_TRY(check_dtype(dtype));
+  if (n_experts < 1 || n_experts > MOE_MAX_EXPERTS)
+    return fail(MOE_ERR_INVALID_ARG, "n_experts must be in [1, %d], got %d", MOE_MAX_EXPERTS, n_experts);
+  if (top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > n_experts)
+    return fail(MOE_ERR_INVALID_ARG, "top_k must be in [1, min(%d, n_experts)], got %d", MOE_MAX_TOP_K, top_k);
+  if (scoring != MOE_SCORING_SIGMOID && scoring != MOE_SCORING_SOFTMAX)
+    return fail(MOE_ERR_INVALID_ARG, "scoring must be one of moe_scoring, got %d", scoring);
+  return MOE_OK;
+}
+
+int moe_route_topk(const void* logits, int dtype, size_t row_stride, const float* bias, int T, int n_experts,
+                   int top_k, int scoring, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                   float* weights, int32_t* ids, void* stream) {
+  MOE_TRY(check_router(dtype, T, n_experts, top_k, scoring));
+  if (n_group < 1 || n_group > 64 || n_experts % n_group)
+    return fail(MOE_ERR_INVALID_ARG, "n_group must be in [1, 64] and divide %d experts, got %d", n_experts, n_group);
+  if (topk_group < 1 || topk_group > n_group)
+    return fail(MOE_ERR_INVALID_ARG, "topk_group must be in [1, n_group], got %d", topk_group);
+  if (group_top != 1 && group_top != 2)
+    return fail(MOE_ERR_INVALID_ARG, "group_top must be 1 or 2, got %d", group_top);
+  if (top_k > topk_group * (n_experts / n_group))
+    return fail(MOE_ERR_INVALID_ARG, "top_k = %d exceeds the %d experts of the kept groups", top_k,
+                topk_group * (n_experts / n_group));
+  if (T == 0) return MOE_OK;
+  MOE_TRY(check_element_ptr(logits, dtype_bytes(dtype), "logits"));
+  if (bias) MOE_TRY(check_element_ptr(bias, 4, "bias"));
+  MOE_TRY(check_element_ptr(weights, 4, "weights"));
+  MOE_TRY(check_element_ptr(ids, 4, "ids"));
+  return hip_status(moe::launch_route_topk(logits, dtype, row_stride, bias, T, n_experts, top_k,
+                                           scoring == MOE_SCORING_SOFTMAX, n_group, topk_group, group_top,
+                                           renormalize, scale, weights, ids, reinterpret_cast<hipStream_t>(stream)),
+                    "route_topk_kernel launch");
+}
+
+int moe_route_topk_backward(const float* grad_weights, const void* logits, int dtype, size_t row_stride,
+                            const int32_t* ids, int T, int n_experts, int top_k, int scoring, int renormalize,
+                            float scale, void* grad_logits, void* stream) {
+  MOE_TRY(check_router(dtype, T, n_experts, top_k, scoring));
+  if (T == 0) return MOE_OK;
+  MOE_TRY(check_element_ptr(grad_weights, 4, "grad_weights"));
+  MOE_TRY(check_element_ptr(logits, dtype_bytes(dtype), "logits"));
+  MOE_TRY(check_element_ptr(ids, 4, "ids"));
+  MOE_TRY(check_ptr(grad_logits, "grad_logits"));
+  return hip_status(moe::launch_route_topk_backward(grad_weights, logits, dtype, row_stride, ids, T, n_experts, top_k,
+                                                    scoring == MOE_SCORING_SOFTMAX, renormalize, scale, grad_logits,
+                                                    reinterpret_cast<hipStream_t>(stream)),
+                    "route_topk_backward_kernel launch");
+}
+
+static int check_blocks(int K, const char* name) {
+  if (K < moe::BLK || K % moe::BLK || K > MOE_MAX_W4_DIM)
+    return fail(MOE_ERR_INVALID_ARG, "%s must be a multiple of %d in [%d, %d], got %d", name, moe::BLK, moe::BLK,
+                MOE_MAX_W4_DIM, K);
+  return MOE_OK;
+}
+
+int moe_quant_act(const void* x, int dtype, size_t row_stride, int T, int K, void* codes, float* scale,
+                  void* stream) {
+  if (T < 0 || T > MOE_MAX_T) return fail(MOE_ERR_INVALID_ARG, "T must be in [0, %d], got %d", MOE_MAX_T, T);
+  MOE_TRY(check_dtype(dtype));
+  MOE_TRY(check_blocks(K, "K"));
+  if (row_stride * dtype_bytes(dtype) % 16)
+    return fail(MOE_ERR_INVALID_ARG, "rows must be a multiple of 16 bytes apart, got %zu elements", row_stride);
+  if (T == 0) return MOE_OK;
+  MOE_TRY(check_ptr(x, "x"));
+  MOE_TRY(check_ptr(codes, "codes"));
+  MOE_TRY(check_ptr(scale, "scale"));
+  return hip_status(moe::launch_quant_act(x, dtype, row_stride, T, K, static_cast<uint8_t*>(codes), scale,
+                                          reinterpret_cast<hipStream_t>(stream)),
+                    "quant_act_kernel launch");
+}
+
+int moe_quantize_w4(const void* w, int dtype, size_t groups, void* codes, void* scales, void* stream) {
+  MOE_TRY(check_dtype(dtype));
+  if (groups > MOE_MAX_W4_GROUPS)
+    return fail(MOE_ERR_INVALID_ARG, "groups must be at most %zu, got %zu", (size_t)MOE_MAX_W4_GROUPS, groups);
+  if (groups == 0) return MOE_OK;
+  MOE_TRY(check_ptr(w, "w"));
+  MOE_TRY(check_ptr(codes, "codes"));
+  MOE_TRY(check_ptr(scales, "scales"));
+  return hip_status(moe::launch_quantize_w4(w, dtype, groups, static_cast<uint8_t*>(codes),
+                                            static_cast<uint8_t*>(scales), reinterpret_cast<hipStream_t>(stream)),
+                    "quantize_w4_kernel launch");
+}
+
+static int check_matrix(int N, int K) {
+  if (N < 1 || N > MOE_MAX_W4_DIM)
+    return fail(MOE_ERR_INVALID_ARG, "N must be in [1, %d], got %d", MOE_MAX_W4_DIM, N);
+  return check_blocks(K, "K");
+}
+
+size_t moe_packed_w4_bytes(int N, int K) {
+  if (N < 1 || N > MOE_MAX_W4_DIM || K < moe::BLK || K % moe::BLK || K > MOE_MAX_W4_DIM) return 0;
+  return moe::w4_packed_bytes(N, K);
+}
+
+static int pack_w4_common(const void* codes, const void* scales, const void* packed, int n, int N, int K, bool unpack,
+                          void* stream) {
+  if (n < 0) return fail(MOE_ERR_INVALID_ARG, "n must be >= 0, got %d", n);
+  MOE_TRY(check_matrix(N, K));
+  if ((size_t)n * moe::w4_packed_bytes(N, K) > ((size_t)1 << 36))
+    return fail(MOE_ERR_INVALID_ARG, "%d matrices of [%d, %d] pack to more than 2^36 bytes", n, N, K);
+  if (n == 0) return MOE_OK;
+  MOE_TRY(check_ptr(codes, "codes"));
+  MOE_TRY(check_ptr(scales, "scales"));
+  MOE_TRY(check_ptr(packed, "packed"));
+  return hip_status(moe::launch_pack_w4(const_cast<uint8_t*>(static_cast<const uint8_t*>(codes)),
+                                        const_cast<uint8_t*>(static_cast<const uint8_t*>(scales)),
+                                        const_cast<uint8_t*>(static_cast<const uint8_t*>(packed)), n, N, K, unpack,
+                                        reinterpret_cast<hipStream_t>(stream)),
+                    "pack_w4_kernel launch");
+}
+
+int moe_pack_w4(const void* codes, const void* scales, void* packed, int n, int N, int K, void* stream) {
+  return pack_w4_common(codes, scales, packed, n, N, K, false, stream);
+}
+int moe_unpack_w4(const void* packed, void* codes, void* scales, int n, int N, int K, void* stream) {
+  return pack_w4_common(codes, scales, packed, n, N, K, true, stream);
+}
+
+int moe_linear_w4(const void* x, const float* x_scale, const void* packed, int T, int N, int K, void* out_bf16,
+                  void* stream) {
+  if (T < 0 || T > MOE_MAX_T) return fail(MOE_ERR_INVALID_ARG, "T must be in [0, %d], got %d", MOE_MAX_T, T);
+  MOE_TRY(check_matrix(N, K));
+  if (T == 0) return MOE_OK;
+  MOE_TRY(check_ptr(x, "x"));
+  MOE_TRY(check_ptr(x_scale, "x_scale"));
+  MOE_TRY(check_ptr(packed, "packed"));
+  MOE_TRY(check_ptr(out_bf16, "out_bf16"));
+  return hip_status(moe::launch_linear_w4(static_cast<const uint8_t*>(x), x_scale,
+                                          static_cast<const uint8_t*>(packed), T, N, K,
+                                          static_cast<uint16_t*>(out_bf16), reinterpret_cast<hipStream_t>(stream)),
+                    "linear_w4_kernel launch");
+}
+
+static int check_experts_w4(int T, int hidden, int inter, int e_local, int top_k) {
+  if (T < 0 || T > MOE_MAX_T) return fail(MOE_ERR_INVALID_ARG, "T must be in [0, %d], got %d", MOE_MAX_T, T);
+  MOE_TRY(check_blocks(hidden, "hidden"));
+  MOE_TRY(check_blocks(inter, "inter"));
+  if (2 * inter > MOE_MAX_W4_DIM)
+    return fail(MOE_ERR_INVALID_ARG, "inter must be at most %d, got %d", MOE_MAX_W4_DIM / 2, inter);
+  if (e_local < 1 || e_local > MOE_MAX_EXPERTS)
+    return fail(MOE_ERR_INVALID_ARG, "e_local must be in [1, %d], got %d", MOE_MAX_EXPERTS, e_local);
+  if (top_k < 1 || top_k > MOE_MAX_TOP_K)
+    return fail(MOE_ERR_INVALID_ARG, "top_k must be in [1, %d], got %d", MOE_MAX_TOP_K, top_k);
+  return MOE_OK;
+}
+
+size_t moe_experts_w4_workspace_bytes(int T, int hidden, int inter, int e_local, int top_k) {
+  if (check_experts_w4(T, hidden, inter, e_local, top_k) != MOE_OK) return 0;
+  return moe::experts_w4_workspace(T, hidden, inter, e_local, top_k);
+}
+
+int moe_experts_w4(const void* x, const float* x_scale, const void* w13_packed, const void* w2_packed,
+                   const int32_t* ids, const float* weights, int T, int hidden, int inter, int e_local, int top_k,
+                   int local_expert_offset, void* workspace, size_t workspace_bytes, void* out_bf16, void* stream) {
+  MOE_TRY(check_experts_w4(T, hidden, inter, e_local, top_k));
+  if (local_expert_offset < 0 || local_expert_offset > (1 << 30))
+    return fail(MOE_ERR_INVALID_ARG, "local_expert_offset must be in [0, 2^30], got %d", local_expert_offset);
+  if (T == 0) return MOE_OK;
+  MOE_TRY(check_ptr(x, "x"));
+  MOE_TRY(check_ptr(x_scale, "x_scale"));
+  MOE_TRY(check_ptr(w13_packed, "w13_packed"));
+  MOE_TRY(check_ptr(w2_packed, "w2_packed"));
+  MOE_TRY(check_element_ptr(ids, 4, "ids"));
+  MOE_TRY(check_element_ptr(weights, 4, "weights"));
+  MOE_TRY(check_ptr(workspace, "workspace"));
+  MOE_TRY(check_ptr(out_bf16, "out_bf16"));
+  const size_t need = moe::experts_w4_workspace(T, hidden, inter, e_local, top_k);
+  if (workspace_bytes < need)
+    return fail(MOE_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu", workspace_bytes, need);
+  const moe::ExpertsW4 a = {static_cast<const uint8_t*>(x),          x_scale,
+                            static_cast<const uint8_t*>(w13_packed), static_cast<const uint8_t*>(w2_packed),
+                            ids, weights, T, hidden, inter, e_local, top_k, local_expert_offset,
+                            static_cast<uint16_t*>(out_bf16)};
+  return hip_status(moe::launch_experts_w4(a, static_cast<uint8_t*>(workspace), reinterpret_cast<hipStream_t>(stream)),
+                    "experts_w4 launch");
+}
+
 int moe_mfma_tiles(const void* a, const void* b, float* d, int n, void* stream) {
   if (n < 0) return fail(MOE_ERR_INVALID_ARG, "n must be >= 0, got %d", n);
   if (n == 0) return MOE_OK;

@@ -119,6 +119,9 @@ __device__ __forceinline__ uint32_t cvt4_e4m3(float a, float b, float c, float d
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
 
+// Element types of the operators that take several (moe_dtype of the C ABI).
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+
 // Flag in route_token: the route is its token's only local route (the GEMM2
 // kernels then write the token's output row, and the combine skips it).
 constexpr int SINGLE_ROUTE_BIT = (int)0x80000000u;

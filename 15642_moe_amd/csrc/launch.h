@@ -88,6 +88,39 @@ hipError_t launch_pack_router(const uint8_t* w, uint8_t* packed, bool unpack, hi
 hipError_t launch_router_quant(const uint8_t* hidden_bf16, const uint8_t* router_packed, int T, float* partial,
                                float* logits, uint8_t* hidden_fp8, float* hidden_scale, hipStream_t stream);
 
+// General router and its gradient (router.hip); dtype DT_* of logits and
+// grad_logits, row_stride in elements.
+hipError_t launch_route_topk(const void* logits, int dtype, size_t row_stride, const float* bias, int T, int E, int k,
+                             int softmax, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                             float* weights, int32_t* ids, hipStream_t stream);
+hipError_t launch_route_topk_backward(const float* grad, const void* logits, int dtype, size_t row_stride,
+                                      const int32_t* ids, int T, int E, int k, int softmax, int renormalize,
+                                      float scale, void* grad_logits, hipStream_t stream);
+
+// 4-bit weights (w4.hip): layout and quantisation of n matrices [N, K], the
+// activation quantiser, the dense product and the experts' products.
+size_t w4_packed_bytes(int N, int K);
+hipError_t launch_pack_w4(uint8_t* codes, uint8_t* scales, uint8_t* packed, int n, int N, int K, bool unpack,
+                          hipStream_t stream);
+hipError_t launch_quantize_w4(const void* w, int dtype, size_t groups, uint8_t* codes, uint8_t* scales,
+                              hipStream_t stream);
+hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, int K, uint8_t* codes, float* scale,
+                            hipStream_t stream);
+hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* packed, int T, int N, int K,
+                            uint16_t* out, hipStream_t stream);
+struct ExpertsW4 {
+  const uint8_t* x;      // e4m3 [T, H]
+  const float* xs;       // [H / 128, T]
+  const uint8_t* w13;    // packed [e_local][2 I, H]
+  const uint8_t* w2;     // packed [e_local][H, I]
+  const int32_t* ids;    // [T, k]
+  const float* weights;  // [T, k]
+  int T, H, I, e_local, k, offset;
+  uint16_t* out;  // bf16 [T, H]
+};
+size_t experts_w4_workspace(int T, int H, int I, int e_local, int k);
+hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* workspace, hipStream_t stream);
+
 hipError_t launch_mfma_tiles(const uint8_t* A, const uint8_t* B, float* D, int n, hipStream_t stream);
 // FP8 MFMA loop of `grid` workgroups of MFMA_CEILING_THREADS threads: out
 // [grid * MFMA_CEILING_THREADS] fp32, clocks [grid][2] (100 MHz ticks, shader

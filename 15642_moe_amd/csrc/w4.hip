@@ -1,0 +1,717 @@
+// 4-bit weights: OCP MXFP4 (e2m1 codes, one e8m0 scale per 32 elements of K) on
+// block-scaled e4m3 activations (one fp32 scale per 128 elements of K).
+//
+//   y[t, n] = sum_kb xs[kb, t] * sum_{k in block kb} x[t, k] * 2^(sc[n, k/32] - 127) * e2m1(code[n, k])
+//
+// The inner sum of a 128-block is one v_mfma_scale_f32_16x16x128_f8f6f4 with
+// the weights as the fp4 A operand, whose e8m0 scales the instruction applies,
+// and the activations as the e4m3 B operand: no dequantisation, and one
+// fp32 multiply-add per output and K-block for the activation scale.
+//
+// What bounds the products at few tokens is the weights' stream, 4.25 bits
+// each: half of the FP8 layer's bytes.
+#include "common.h"
+#include "launch.h"
+#include "w4.h"
+
+#include <type_traits>
+
+namespace moe {
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Workgroups of a launch whose kernel loops over what is left (a launch's
+// threads have to stay below 2^32).
+constexpr size_t MAX_GRID = (size_t)1 << 20;
+
+// ---------------------------------------------------------------------------
+// Layout.  A thread per 16 bytes of codes (and, of them, the first of a
+// K-block per scale byte).
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256)
+pack_w4_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ packed, int N, int K,
+               size_t units, int unpack) {
+  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;  // (matrix and 16-row tile, chunk, K-block, lane)
+  if (u >= units) return;
+  const int lane = u & 63, b = (u >> 6) & 3;
+  const int KC = w4_chunks(K), NT = w4_tiles(N);
+  const size_t q = u >> 8;  // packed chunk
+  const int c = (int)(q % KC), tile = (int)(q / KC % NT);
+  const size_t m = q / KC / NT;
+  const int row = tile * 16 + (lane & 15), g = lane >> 4, kb = c * W4_CHUNK_BLOCKS + b;
+  const bool there = row < N && kb * BLK < K;
+  uint8_t* pc = packed + q * W4_CHUNK_BYTES + b * W4_BLOCK_BYTES + lane * 16;
+  uint8_t* ps = packed + q * W4_CHUNK_BYTES + W4_CHUNK_BLOCKS * W4_BLOCK_BYTES + lane * 4 + b;
+  const size_t src = (m * N + (there ? row : 0)) * (size_t)(K / 2) + (size_t)(there ? kb : 0) * (BLK / 2) + g * 16;
+  const size_t ssrc = (m * N + (there ? row : 0)) * (size_t)(K / 32) + (size_t)(there ? kb : 0) * (BLK / 32) + g;
+  if (unpack) {
+    if (!there) return;
+    *reinterpret_cast<uint4*>(codes + src) = *reinterpret_cast<const uint4*>(pc);
+    scales[ssrc] = *ps;
+  } else {
+    // Padding rows and K-blocks: zero codes at scale 1.
+    *reinterpret_cast<uint4*>(pc) = there ? *reinterpret_cast<const uint4*>(codes + src) : make_uint4(0, 0, 0, 0);
+    *ps = there ? scales[ssrc] : (uint8_t)127;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* base, size_t i, float (&f)[8]) {
+  if constexpr (DT == DT_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == DT_BF16) {
+        f[2 * j] = __builtin_bit_cast(float, u[j] << 16);
+        f[2 * j + 1] = __builtin_bit_cast(float, u[j] & 0xFFFF0000u);
+      } else {
+        f[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)u[j]);
+        f[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[j] >> 16));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// MXFP4 of a matrix: the shared exponent of 32 elements is that of their
+// largest magnitude less 2 (the OCP rule: it lands in [4, 8), of which e2m1
+// reaches 6), codes rounded to nearest, ties to even, saturating.  A group with
+// an infinity or NaN gets the NaN scale.  Four threads a group, 8 elements each.
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ void __launch_bounds__(256)
+quantize_w4_kernel(const void* __restrict__ w, size_t groups, uint8_t* __restrict__ codes,
+                   uint8_t* __restrict__ scales) {
+  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t grp = u >> 2;
+  const bool active = grp < groups;
+  float f[8];
+  load8<DT>(w, (active ? u : 0) * 8, f);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7FFFFFFFu);  // NaN above inf
+  m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+  const bool bad = m >= 0x7F800000u;
+  // e8m0 = (exponent field of the maximum) - 2, at least 0: a maximum below
+  // 2^-125 keeps the smallest scale, 2^-127.
+  const int ex = max((int)(m >> 23) - 2, 0);
+  uint32_t packed = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = ldexpf(fabsf(f[j]), 127 - ex);
+    uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
+    c |= (__float_as_uint(f[j]) >> 28) & 8u;
+    packed |= (bad ? 0u : c) << (4 * j);
+  }
+  if (!active) return;
+  reinterpret_cast<uint32_t*>(codes)[u] = packed;
+  if ((u & 3) == 0) scales[grp] = bad ? (uint8_t)255 : (uint8_t)ex;
+}
+
+// ---------------------------------------------------------------------------
+// Activations: per (row, 128 columns) scale = max(amax / 448, 1e-8), code =
+// e4m3(clamp(x / scale, +-448)), the rule of the producer and of the experts'
+// own requantisation.  16 lanes a block, 8 columns each.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint2 quant8(const float (&f)[8], float& sc) {
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  sc = fmaxf(m / E4M3_MAX, 1.0e-8f);
+  auto q = [&](float x) {  // a NaN (an infinity in its block) stays one
+    const float v = x / sc;
+    return v > E4M3_MAX ? E4M3_MAX : v < -E4M3_MAX ? -E4M3_MAX : v;
+  };
+  uint2 o;
+  o.x = cvt4_e4m3(q(f[0]), q(f[1]), q(f[2]), q(f[3]));
+  o.y = cvt4_e4m3(q(f[4]), q(f[5]), q(f[6]), q(f[7]));
+  return o;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256)
+quant_act_kernel(const void* __restrict__ x, size_t row_stride, int T, int KB, uint8_t* __restrict__ codes,
+                 float* __restrict__ scale) {
+  const size_t n = (size_t)T * KB;  // (row, block)
+  const int sub = threadIdx.x & 15;
+  for (size_t u0 = (size_t)blockIdx.x * 16; u0 < n; u0 += (size_t)gridDim.x * 16) {
+    const size_t u = u0 + (threadIdx.x >> 4);
+    const bool active = u < n;
+    const size_t t = active ? u / KB : 0;
+    const int kb = active ? (int)(u % KB) : 0;
+    float f[8], sc;
+    load8<DT>(x, t * row_stride + (size_t)kb * BLK + sub * 8, f);
+    const uint2 o = quant8(f, sc);
+    if (active) {
+      *reinterpret_cast<uint2*>(codes + (t * KB + kb) * BLK + sub * 8) = o;
+      if (sub == 0) scale[(size_t)kb * T + t] = sc;
+    }
+  }
+}
+
+// The same for the experts' SwiGLU output: Cf [R, I] -> Cq [R, I], Cs [R, I / 128].
+__global__ void __launch_bounds__(256)
+requant_kernel(const float* __restrict__ Cf, const int32_t* __restrict__ n_routes, int IB, uint8_t* __restrict__ Cq,
+               float* __restrict__ Cs) {
+  const size_t n = (size_t)*n_routes * IB;
+  const int sub = threadIdx.x & 15;
+  for (size_t u0 = (size_t)blockIdx.x * 16; u0 < n; u0 += (size_t)gridDim.x * 16) {
+    const size_t u = u0 + (threadIdx.x >> 4);
+    const bool active = u < n;
+    float f[8], sc;
+    load8<DT_F32>(Cf, (active ? u : 0) * BLK + sub * 8, f);
+    const uint2 o = quant8(f, sc);
+    if (active) {
+      *reinterpret_cast<uint2*>(Cq + u * BLK + sub * 8) = o;
+      if (sub == 0) Cs[u] = sc;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The products.  A wave multiplies NT 16-row weight tiles with FR fragments of
+// 16 activation rows over its share of the chunks of 512 K elements; the
+// waves of a workgroup split the chunks, and their sums are added in K order
+// through LDS.
+// ---------------------------------------------------------------------------
+template <int B>
+__device__ __forceinline__ v4f mfma_w4(const u32x4& a, const v8i& x, int scale, const v4f& c) {
+  v8i aw{};
+  aw[0] = (int)a[0]; aw[1] = (int)a[1]; aw[2] = (int)a[2]; aw[3] = (int)a[3];
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aw, x, c, 4, 0, B, scale, 0, 127);
+}
+
+template <int N, int I0 = 0, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I0 < N) {
+    f(std::integral_constant<int, I0>{});
+    static_for<N, I0 + 1>(f);
+  }
+}
+
+template <int NT, int FR>
+struct Stream {
+  const uint8_t* w[NT];   // packed tiles, this lane's 16 bytes of the first K-block
+  const uint8_t* x[FR];   // this lane's activation row, at its 16 bytes of the first K-block
+  const float* xs[FR];    // that row's scale of the first K-block
+  size_t xs_stride;       // from one K-block's scale to the next
+  u32x4 a[NT][4];
+  int sc[NT];
+  v4f acc[NT][FR];
+
+  __device__ __forceinline__ void load(int c) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* p = w[n] + (size_t)c * W4_CHUNK_BYTES;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        a[n][b] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + b * W4_BLOCK_BYTES));
+      sc[n] = __builtin_nontemporal_load(
+          reinterpret_cast<const int*>(p + W4_CHUNK_BLOCKS * W4_BLOCK_BYTES - 12 * (threadIdx.x & 63)));
+    }
+  }
+  // Chunks c0 .. c1 - 1 of KB K-blocks in all.
+  __device__ __forceinline__ void run(int c0, int c1, int KB) {
+    const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int f = 0; f < FR; ++f) acc[n][f] = zero4;
+    if (c0 >= c1) return;
+    load(c0);
+    for (int c = c0; c < c1; ++c) {
+      u32x4 ca[NT][4];
+      int csc[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        csc[n] = sc[n];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) ca[n][b] = a[n][b];
+      }
+      if (c + 1 < c1) load(c + 1);
+      static_for<4>([&](auto bc) __attribute__((always_inline)) {
+        constexpr int b = decltype(bc)::value;
+        const int kb = c * W4_CHUNK_BLOCKS + b;
+        if (kb < KB) {
+#pragma unroll
+          for (int f = 0; f < FR; ++f) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK);
+            const u32x4 hi = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK + 64);
+            const float s = xs[f][(size_t)kb * xs_stride];
+            const v8i xb = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][f] += mfma_w4<b>(ca[n][b], xb, csc[n], zero4) * s;
+          }
+        }
+      });
+    }
+  }
+  // The workgroup's sums, entry (n, f) in the registers of the wave that owns
+  // it: `own(entry)` is called for the entries of this wave, after the waves'
+  // parts have been added in K order.  Entries come as groups of G tiles (a
+  // gate and an up tile for GEMM1): group p holds tiles p, p + NT / G, ...
+  template <int G, class F>
+  __device__ __forceinline__ void reduce(v4f* lds, int wave, int waves, F&& own) {
+    const int lane = threadIdx.x & 63;
+    constexpr int NP = NT / G;
+    if (waves == 1) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int f = 0; f < FR; ++f) {
+          v4f y[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) y[g] = acc[p + g * NP][f];
+          own(p, f, y);
+        }
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int f = 0; f < FR; ++f) lds[((wave * NT + n) * FR + f) * 64 + lane] = acc[n][f];
+    __syncthreads();
+    for (int i = wave; i < NP * FR; i += waves) {
+      const int p = i / FR, f = i % FR;
+      v4f y[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        y[g] = lds[((p + g * NP) * FR + f) * 64 + lane];
+        for (int k = 1; k < waves; ++k) y[g] += lds[((k * NT + p + g * NP) * FR + f) * 64 + lane];
+      }
+      own(p, f, y);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  auto one = [](float v) -> uint32_t { return v == v ? bf16_rne(v) : 0x7FC0u; };
+  return one(a) | one(b) << 16;
+}
+
+__device__ __forceinline__ int chunk_begin(int KC, int wave, int waves) { return KC * wave / waves; }
+
+// y[t, n]: workgroup (row tiles nt*NT .., token group tg).
+template <int NT, int FR>
+__global__ void __launch_bounds__(512)
+linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
+                                 const uint8_t* __restrict__ packed, int T, int N, int K,
+                                 uint16_t* __restrict__ out) {
+  extern __shared__ v4f s_part[];
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int KC = w4_chunks(K), tiles = w4_tiles(N), KB = K / BLK;
+  const int t0 = blockIdx.y * (16 * FR), n0 = blockIdx.x * NT;
+  Stream<NT, FR> st;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    st.w[n] = packed + (size_t)min(n0 + n, tiles - 1) * KC * W4_CHUNK_BYTES + lane * 16;
+#pragma unroll
+  for (int f = 0; f < FR; ++f) {
+    const int t = min(t0 + 16 * f + (lane & 15), T - 1);  // padding columns reread the last row
+    st.x[f] = x + (size_t)t * K + 16 * (lane >> 4);
+    st.xs[f] = xs + t;
+  }
+  st.xs_stride = T;
+  st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
+  st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+    const int t = t0 + 16 * f + (lane & 15), n = (n0 + p) * 16 + 4 * (lane >> 4);
+    if (t >= T || n >= N) return;
+    uint16_t* dst = out + (size_t)t * N + n;
+    const uint32_t lo = bf16_pair(y[0][0], y[0][1]), hi = bf16_pair(y[0][2], y[0][3]);
+    if ((N & 3) == 0) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+      dst[0] = (uint16_t)lo;
+      if (n + 1 < N) dst[1] = (uint16_t)(lo >> 16);
+      if (n + 2 < N) dst[2] = (uint16_t)hi;
+      if (n + 3 < N) dst[3] = (uint16_t)(hi >> 16);
+    }
+  });
+}
+
+// ---------------------------------------------------------------------------
+// The experts.  Dispatch: a counting sort of the local picks into routes, expert
+// by expert, and a list of route tiles of `bm` routes.  A pick's place among its
+// expert's routes is taken from an atomic and may differ from run to run; no
+// result does, since every route is computed by itself and a token's routes are
+// added in the order of its picks.
+// ---------------------------------------------------------------------------
+struct Routes {
+  int32_t* offsets;      // [e_local + 1] first route of each expert; the last: their number
+  int32_t* n_tiles;      // [1]
+  int4* tiles;           // {expert, first route, routes, 0}
+  int32_t* route_pick;   // [T k]
+  int32_t* pick_route;   // [T k], -1 for picks of other experts
+  int32_t* chunk_counts; // [chunks][e_local]
+};
+constexpr int SORT_THREADS = 1024, SORT_CHUNK = 8192;  // picks per workgroup
+constexpr int MAX_EXPERTS = 1024;
+
+// s_scan[0 .. n) exclusive prefix sums of v over the threads; returns this
+// thread's, `total` the sum.
+__device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int inc = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  __syncthreads();
+  if (lane == 63) s_wave[wave] = inc;
+  __syncthreads();
+  int base = 0;
+  total = 0;
+  for (int w = 0; w < SORT_THREADS / 64; ++w) {
+    base += w < wave ? s_wave[w] : 0;
+    total += s_wave[w];
+  }
+  return base + inc - v;
+}
+
+// Offsets and the tile list from expert `threadIdx.x`'s count; s_off / s_tp
+// [e_local] receive the first routes and tiles.
+__device__ __forceinline__ void publish_tiles(int cnt, int e_local, int bm, const Routes& r, int* s_off, int* s_tp,
+                                              int* s_cnt, int* s_wave) {
+  const int e = threadIdx.x;
+  int total, tiles;
+  const int off = block_scan(cnt, s_wave, total);
+  const int tp = block_scan((cnt + bm - 1) / bm, s_wave, tiles);
+  if (e < e_local) {
+    s_off[e] = off;
+    s_tp[e] = tp;
+    s_cnt[e] = cnt;
+    r.offsets[e] = off;
+  }
+  if (e == 0) {
+    r.offsets[e_local] = total;
+    *r.n_tiles = tiles;
+  }
+  __syncthreads();
+  for (int i = e; i < tiles; i += SORT_THREADS) {
+    int lo = 0, hi = e_local - 1;  // the last expert whose first tile is at most i (and which has any)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_tp[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    const int m0 = (i - s_tp[lo]) * bm;
+    r.tiles[i] = make_int4(lo, s_off[lo] + m0, min(bm, s_cnt[lo] - m0), 0);
+  }
+}
+
+// All picks by one workgroup.
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_small_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, int bm, Routes r) {
+  __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_pos[MAX_EXPERTS], s_wave[16];
+  const int tid = threadIdx.x;
+  s_pos[tid] = 0;
+  __syncthreads();
+  for (int p = tid; p < picks; p += SORT_THREADS) {
+    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
+    if (e < (unsigned)e_local && ids[p] >= 0) atomicAdd(&s_pos[e], 1);
+  }
+  __syncthreads();
+  publish_tiles(tid < e_local ? s_pos[tid] : 0, e_local, bm, r, s_off, s_tp, s_cnt, s_wave);
+  __syncthreads();
+  s_pos[tid] = tid < e_local ? s_off[tid] : 0;
+  __syncthreads();
+  for (int p = tid; p < picks; p += SORT_THREADS) {
+    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
+    int at = -1;
+    if (e < (unsigned)e_local && ids[p] >= 0) {
+      at = atomicAdd(&s_pos[e], 1);
+      r.route_pick[at] = p;
+    }
+    r.pick_route[p] = at;
+  }
+}
+
+// The same over several workgroups: counts of each SORT_CHUNK picks, ...
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_count_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, Routes r) {
+  __shared__ int s_cnt[MAX_EXPERTS];
+  const int tid = threadIdx.x;
+  s_cnt[tid] = 0;
+  __syncthreads();
+  const int p1 = min(picks, ((int)blockIdx.x + 1) * SORT_CHUNK);
+  for (int p = blockIdx.x * SORT_CHUNK + tid; p < p1; p += SORT_THREADS) {
+    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
+    if (e < (unsigned)e_local && ids[p] >= 0) atomicAdd(&s_cnt[e], 1);
+  }
+  __syncthreads();
+  if (tid < e_local) r.chunk_counts[(size_t)blockIdx.x * e_local + tid] = s_cnt[tid];
+}
+// ... each chunk's first places, ...
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_scan_kernel(int chunks, int e_local, int bm, Routes r) {
+  __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_wave[16];
+  const int e = threadIdx.x;
+  int cnt = 0;
+  if (e < e_local)
+    for (int c = 0; c < chunks; ++c) cnt += r.chunk_counts[(size_t)c * e_local + e];
+  publish_tiles(cnt, e_local, bm, r, s_off, s_tp, s_cnt, s_wave);
+  if (e < e_local) {
+    int at = s_off[e];
+    for (int c = 0; c < chunks; ++c) {
+      const size_t i = (size_t)c * e_local + e;
+      const int n = r.chunk_counts[i];
+      r.chunk_counts[i] = at;
+      at += n;
+    }
+  }
+}
+// ... and the places.
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_place_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, Routes r) {
+  __shared__ int s_pos[MAX_EXPERTS];
+  const int tid = threadIdx.x;
+  if (tid < e_local) s_pos[tid] = r.chunk_counts[(size_t)blockIdx.x * e_local + tid];
+  __syncthreads();
+  const int p1 = min(picks, ((int)blockIdx.x + 1) * SORT_CHUNK);
+  for (int p = blockIdx.x * SORT_CHUNK + tid; p < p1; p += SORT_THREADS) {
+    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
+    int at = -1;
+    if (e < (unsigned)e_local && ids[p] >= 0) {
+      at = atomicAdd(&s_pos[e], 1);
+      r.route_pick[at] = p;
+    }
+    r.pick_route[p] = at;
+  }
+}
+
+// GEMM1 and SwiGLU of (route tile, NP pairs of 16 gate and 16 up rows): rows
+// [0, I) of W13 multiply, SiLU takes rows [I, 2 I).  Workgroups past the last
+// tile end at once.
+template <int NP, int FR>
+__global__ void __launch_bounds__(512)
+experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
+  extern __shared__ v4f s_part[];
+  const int slices = a.I / 16 / NP;
+  const int j = blockIdx.x % slices, n_tiles = *r.n_tiles;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int KC = w4_chunks(a.H), KB = a.H / BLK, tiles = 2 * a.I / 16;
+  for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
+    if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
+    const int4 tile = r.tiles[i];
+    Stream<2 * NP, FR> st;
+#pragma unroll
+    for (int n = 0; n < 2 * NP; ++n) {
+      const int row = j * NP + (n < NP ? n : a.I / 16 + n - NP);
+      st.w[n] = a.w13 + ((size_t)tile.x * tiles + row) * KC * W4_CHUNK_BYTES + lane * 16;
+    }
+#pragma unroll
+    for (int f = 0; f < FR; ++f) {
+      const int t = r.route_pick[tile.y + min(16 * f + (lane & 15), tile.z - 1)] / a.k;
+      st.x[f] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
+      st.xs[f] = a.xs + t;
+    }
+    st.xs_stride = a.T;
+    st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
+    st.template reduce<2>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+      const int m = 16 * f + (lane & 15);
+      if (m >= tile.z) return;
+      float4 c;
+      c.x = y[1][0] / (1.0f + __expf(-y[1][0])) * y[0][0];
+      c.y = y[1][1] / (1.0f + __expf(-y[1][1])) * y[0][1];
+      c.z = y[1][2] / (1.0f + __expf(-y[1][2])) * y[0][2];
+      c.w = y[1][3] / (1.0f + __expf(-y[1][3])) * y[0][3];
+      *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + (j * NP + p) * 16 + 4 * (lane >> 4)) = c;
+    });
+  }
+}
+
+// GEMM2 of (route tile, NT 16-row tiles of W2), times the pick's weight.
+template <int NT, int FR>
+__global__ void __launch_bounds__(512)
+experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
+                                     const float* __restrict__ Cs, float* __restrict__ Y) {
+  extern __shared__ v4f s_part[];
+  const int slices = a.H / 16 / NT;
+  const int j = blockIdx.x % slices, n_tiles = *r.n_tiles;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int KC = w4_chunks(a.I), KB = a.I / BLK, tiles = a.H / 16;
+  for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
+    if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
+    const int4 tile = r.tiles[i];
+    Stream<NT, FR> st;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      st.w[n] = a.w2 + ((size_t)tile.x * tiles + j * NT + n) * KC * W4_CHUNK_BYTES + lane * 16;
+#pragma unroll
+    for (int f = 0; f < FR; ++f) {
+      const size_t row = tile.y + min(16 * f + (lane & 15), tile.z - 1);
+      st.x[f] = Cq + row * a.I + 16 * (lane >> 4);
+      st.xs[f] = Cs + row * KB;
+    }
+    st.xs_stride = 1;
+    st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
+    st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+      const int m = 16 * f + (lane & 15);
+      if (m >= tile.z) return;
+      const float w = a.weights[r.route_pick[tile.y + m]];
+      *reinterpret_cast<float4*>(Y + (size_t)(tile.y + m) * a.H + (j * NT + p) * 16 + 4 * (lane >> 4)) =
+          make_float4(y[0][0] * w, y[0][1] * w, y[0][2] * w, y[0][3] * w);
+    });
+  }
+}
+
+// out[t] = the sum of its local picks' Y rows, in the order of the picks.
+__global__ void __launch_bounds__(256)
+experts_combine_kernel(const float* __restrict__ Y, const int32_t* __restrict__ pick_route, int H, int k,
+                       uint16_t* __restrict__ out) {
+  const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= H) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j = 0; j < k; ++j) {
+    const int r = pick_route[(size_t)t * k + j];
+    if (r < 0) continue;
+    const float4 y = *reinterpret_cast<const float4*>(Y + (size_t)r * H + c);
+    s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
+  }
+  *reinterpret_cast<uint2*>(out + (size_t)t * H + c) = make_uint2(bf16_pair(s.x, s.y), bf16_pair(s.z, s.w));
+}
+
+struct ExpertsLayout {
+  size_t offsets, n_tiles, tiles, route_pick, pick_route, chunk_counts, cf, cq, cs, y, total;
+};
+// The smallest route tile sets the length of the tile list.
+constexpr int MIN_BM = 16;
+size_t max_tiles(size_t picks, int e_local, int bm) {
+  return (picks < (size_t)e_local ? picks : (size_t)e_local) + picks / bm;
+}
+ExpertsLayout experts_layout(int T, int H, int I, int e_local, int k) {
+  const size_t picks = (size_t)T * k, chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  ExpertsLayout l;
+  l.offsets = take(((size_t)e_local + 1) * 4);
+  l.n_tiles = take(4);
+  l.tiles = take(max_tiles(picks, e_local, MIN_BM) * 16);
+  l.route_pick = take(picks * 4);
+  l.pick_route = take(picks * 4);
+  l.chunk_counts = take(chunks * e_local * 4);
+  l.cf = take(picks * I * 4);
+  l.cq = take(picks * I);
+  l.cs = take(picks * (I / BLK) * 4);
+  l.y = take(picks * H * 4);
+  l.total = at;
+  return l;
+}
+
+}  // namespace
+
+size_t w4_packed_bytes(int N, int K) { return (size_t)w4_tiles(N) * w4_chunks(K) * W4_CHUNK_BYTES; }
+
+hipError_t launch_pack_w4(uint8_t* codes, uint8_t* scales, uint8_t* packed, int n, int N, int K, bool unpack,
+                          hipStream_t stream) {
+  const size_t units = (size_t)n * w4_tiles(N) * w4_chunks(K) * W4_CHUNK_BLOCKS * 64;
+  pack_w4_kernel<<<(unsigned)((units + 255) / 256), 256, 0, stream>>>(codes, scales, packed, N, K, units, unpack);
+  return hipGetLastError();
+}
+
+hipError_t launch_quantize_w4(const void* w, int dtype, size_t groups, uint8_t* codes, uint8_t* scales,
+                              hipStream_t stream) {
+  const unsigned grid = (unsigned)((groups * 4 + 255) / 256);
+  if (dtype == DT_F32) quantize_w4_kernel<DT_F32><<<grid, 256, 0, stream>>>(w, groups, codes, scales);
+  else if (dtype == DT_BF16) quantize_w4_kernel<DT_BF16><<<grid, 256, 0, stream>>>(w, groups, codes, scales);
+  else quantize_w4_kernel<DT_F16><<<grid, 256, 0, stream>>>(w, groups, codes, scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, int K, uint8_t* codes, float* scale,
+                            hipStream_t stream) {
+  const size_t blocks = ((size_t)T * (K / BLK) + 15) / 16;
+  const unsigned grid = (unsigned)(blocks < MAX_GRID ? blocks : MAX_GRID);
+  if (dtype == DT_F32) quant_act_kernel<DT_F32><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
+  else if (dtype == DT_BF16) quant_act_kernel<DT_BF16><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
+  else quant_act_kernel<DT_F16><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* packed, int T, int N, int K,
+                            uint16_t* out, hipStream_t stream) {
+  const int tiles = w4_tiles(N), KC = w4_chunks(K);
+  const int waves = KC < 8 ? KC : 8;
+  auto launch = [&](auto kernel, int nt, int fr) {
+    const dim3 grid((tiles + nt - 1) / nt, (T + 16 * fr - 1) / (16 * fr));
+    kernel<<<grid, 64 * waves, waves > 1 ? waves * nt * fr * 1024 : 0, stream>>>(x, xs, packed, T, N, K, out);
+  };
+  if (T <= 16) launch(linear_w4_kernel<1, 1>, 1, 1);
+  else launch(linear_w4_kernel<2, 2>, 2, 2);
+  return hipGetLastError();
+}
+
+size_t experts_w4_workspace(int T, int H, int I, int e_local, int k) {
+  return experts_layout(T, H, I, e_local, k).total;
+}
+
+hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream) {
+  const ExpertsLayout l = experts_layout(a.T, a.H, a.I, a.e_local, a.k);
+  const Routes r = {reinterpret_cast<int32_t*>(ws + l.offsets),    reinterpret_cast<int32_t*>(ws + l.n_tiles),
+                    reinterpret_cast<int4*>(ws + l.tiles),         reinterpret_cast<int32_t*>(ws + l.route_pick),
+                    reinterpret_cast<int32_t*>(ws + l.pick_route), reinterpret_cast<int32_t*>(ws + l.chunk_counts)};
+  float* Cf = reinterpret_cast<float*>(ws + l.cf);
+  uint8_t* Cq = ws + l.cq;
+  float* Cs = reinterpret_cast<float*>(ws + l.cs);
+  float* Y = reinterpret_cast<float*>(ws + l.y);
+  const int picks = a.T * a.k;
+  const int fr = a.T <= 16 ? 1 : 2, bm = 16 * fr;
+  hipError_t err;
+  if (picks <= SORT_CHUNK) {
+    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, bm, r);
+  } else {
+    const int chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
+    sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    sort_scan_kernel<<<1, SORT_THREADS, 0, stream>>>(chunks, a.e_local, bm, r);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
+  }
+  if ((err = hipGetLastError()) != hipSuccess) return err;
+  const size_t bound = max_tiles(picks, a.e_local, bm);
+  // Workgroups: every tile's slices, or as many tiles' as fit, which then loop.
+  auto grid_of = [&](int slices) {
+    const size_t fit = MAX_GRID / slices > 0 ? MAX_GRID / slices : 1;
+    return (unsigned)((bound < fit ? bound : fit) * slices);
+  };
+  auto waves_of = [](int K) { return w4_chunks(K) < 8 ? w4_chunks(K) : 8; };
+  {
+    const int w = waves_of(a.H);
+    const unsigned grid = grid_of(a.I / 16);
+    if (fr == 1) experts_gemm1_kernel<1, 1><<<grid, 64 * w, w * 2 * 1024, stream>>>(a, r, Cf);
+    else experts_gemm1_kernel<1, 2><<<grid, 64 * w, w * 4 * 1024, stream>>>(a, r, Cf);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+  }
+  const size_t units = (size_t)picks * (a.I / BLK);
+  requant_kernel<<<(unsigned)(units < 16 * 2048 ? (units + 15) / 16 : 2048), 256, 0, stream>>>(Cf, r.offsets + a.e_local,
+                                                                                               a.I / BLK, Cq, Cs);
+  if ((err = hipGetLastError()) != hipSuccess) return err;
+  {
+    const int w = waves_of(a.I);
+    const unsigned grid = grid_of(a.H / 32);
+    if (fr == 1) experts_gemm2_kernel<2, 1><<<grid, 64 * w, w * 2 * 1024, stream>>>(a, r, Cq, Cs, Y);
+    else experts_gemm2_kernel<2, 2><<<grid, 64 * w, w * 4 * 1024, stream>>>(a, r, Cq, Cs, Y);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+  }
+  experts_combine_kernel<<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, stream>>>(Y, r.pick_route, a.H, a.k, a.out);
+  return hipGetLastError();
+}
+
+}  // namespace moe

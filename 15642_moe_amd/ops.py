@@ -242,6 +242,265 @@ def moe_forward(hidden, hidden_scale, W13_packed, W13_scale, W2_packed, W2_scale
                                  rsf, local_offset)[0]
 
 
+# --------------------------------------------------------------------------- general router
+_DTYPES = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}
+
+
+def _rows(name: str, x: torch.Tensor) -> int:
+    """Checks a [T, n] float input and returns its row stride in elements."""
+    _require_device(name, x)
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    _check(x.dim() == 2, f"{name} must be two-dimensional")
+    _check(x.stride(1) == 1 or x.size(1) == 1, f"{name} must be contiguous along its last dimension")
+    return int(x.stride(0)) if x.size(0) > 1 else int(x.size(1))
+
+
+def _check_router(logits, top_k, scoring):
+    stride = _rows("logits", logits)
+    E = int(logits.size(1))
+    if scoring not in capi.SCORING:
+        raise RuntimeError(f"scoring must be one of {sorted(capi.SCORING)}, got {scoring!r}")
+    if not 1 <= E <= capi.MAX_EXPERTS:
+        raise RuntimeError(f"logits must have 1 to {capi.MAX_EXPERTS} experts, got {E}")
+    if not 1 <= top_k <= min(capi.MAX_TOP_K, E):
+        raise RuntimeError(f"top_k must be in [1, {min(capi.MAX_TOP_K, E)}], got {top_k}")
+    return int(logits.size(0)), E, stride
+
+
+def _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale):
+    T, E, stride = _check_router(logits, top_k, scoring)
+    dev = logits.device
+    if bias is not None:
+        _check(bias.dtype == torch.float32 and bias.dim() == 1 and bias.numel() == E and bias.is_contiguous(),
+               f"bias must be float32 [{E}] contiguous")
+        _require_device("bias", bias, dev)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        capi.check(capi.load().moe_route_topk(
+            _ptr(logits), _DTYPES[logits.dtype], stride, _ptr(bias) if bias is not None else None, T, E, top_k,
+            capi.SCORING[scoring], n_group, topk_group, group_top, int(renormalize), scale, _ptr(weights), _ptr(ids),
+            _stream(dev)), "route_topk")
+    return weights, ids
+
+
+def route_topk_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, scoring: str = "sigmoid",
+                        renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """The gradient of route_topk's logits [T, n_experts], in their type, from that of its weights (f32 [T, top_k])
+    and its picks.  Picks outside [0, n_experts) (an unfilled slot's -1) take no part."""
+    _check(ids.dim() == 2 and ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be int32 [T, top_k] contiguous")
+    top_k = int(ids.size(1))
+    T, E, stride = _check_router(logits, top_k, scoring)
+    dev = logits.device
+    _check(ids.size(0) == T, "ids must have a row per token")
+    _check(grad_weights.dtype == torch.float32 and grad_weights.shape == ids.shape and grad_weights.is_contiguous(),
+           "grad_weights must be float32 [T, top_k] contiguous")
+    _require_device("ids", ids, dev)
+    _require_device("grad_weights", grad_weights, dev)
+    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        capi.check(capi.load().moe_route_topk_backward(
+            _ptr(grad_weights), _ptr(logits), _DTYPES[logits.dtype], stride, _ptr(ids), T, E, top_k,
+            capi.SCORING[scoring], int(renormalize), float(scale), _ptr(out), _stream(dev)), "route_topk_backward")
+    return out
+
+
+class _RouteTopK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale):
+        weights, ids = _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale)
+        ctx.save_for_backward(logits, ids)
+        ctx.form = (scoring, renormalize, scale)
+        ctx.mark_non_differentiable(ids)
+        return weights, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_weights, _):
+        logits, ids = ctx.saved_tensors
+        return (route_topk_backward(grad_weights.contiguous(), logits, ids, *ctx.form),) + (None,) * 8
+
+
+def route_topk(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, scoring: str = "sigmoid",
+               n_group: int = 1, topk_group: int | None = None, group_top: int = 2, renormalize: bool = True,
+               scale: float = 1.0):
+    """(weights f32 [T, top_k], ids int32 [T, top_k]) of the experts that each token goes to.
+
+    Scores are sigmoid or softmax of the logits [T, n_experts] (float32, bfloat16 or float16; rows may be strided).
+    Picks go by score + bias: of the `topk_group` best of `n_group` equal groups (a group counts the sum of its
+    `group_top` largest), the `top_k` best experts, ties to the lower index, listed in ascending order.  Weights are the
+    picks' scores, divided by their sum with `renormalize`, times `scale`.
+
+    An expert whose logit (or logit's score + bias) is -inf or NaN is never picked; a slot that no expert fills holds
+    id -1 and weight 0.  The weights are differentiable in the logits; the bias only balances load and takes no
+    gradient.  `experts_w4` takes the result as it is."""
+    topk_group = n_group if topk_group is None else topk_group
+    form = (int(top_k), scoring, int(n_group), int(topk_group), int(group_top), bool(renormalize), float(scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _RouteTopK.apply(logits, None if bias is None else bias.detach(), *form)
+    return _route_topk(logits, bias, *form)
+
+
+# --------------------------------------------------------------------------- 4-bit weights
+W4_GROUP = 32            # elements of K that share an e8m0 scale
+W4_CHUNK_BYTES = 4352    # 16 rows x 512 elements of K, codes and scales
+W4_CHUNK_K = 512
+
+
+def quant_act(x: torch.Tensor):
+    """[T, K] float32, bfloat16 or float16 (K a multiple of 128) -> (e4m3 [T, K], scale f32 [K / 128, T]): the
+    quantisation that router_quant does on its way, for the input of linear_w4 and experts_w4 or moe_forward."""
+    stride = _rows("x", x)
+    T, K = int(x.size(0)), int(x.size(1))
+    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"x must have a multiple of 128 columns, got {K}")
+    _check(T <= capi.MAX_T, f"T must be <= {capi.MAX_T}")
+    _check(stride * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0, "x must have 16-byte aligned rows")
+    codes = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((K // 128, T), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        capi.check(capi.load().moe_quant_act(_ptr(x), _DTYPES[x.dtype], stride, T, K, _ptr(codes), _ptr(scale),
+                                             _stream(x.device)), "quant_act")
+    return codes, scale
+
+
+def quantize_w4(w: torch.Tensor):
+    """A weight [..., N, K] (float32, bfloat16 or float16; K a multiple of 128) to OCP MXFP4: codes uint8
+    [..., N, K / 2] (two e2m1 elements a byte, the lower index in the low half) and e8m0 scales uint8 [..., N, K / 32],
+    for pack_w4.  Round to nearest, ties to even, saturating; a group with an infinity or NaN gets the NaN scale."""
+    _require_device("w", w)
+    if w.dtype not in _DTYPES:
+        raise RuntimeError(f"w must be float32, bfloat16 or float16, got {w.dtype}")
+    _check(w.dim() >= 2 and w.is_contiguous() and w.data_ptr() % 16 == 0, "w must be [..., N, K] contiguous, 16-byte aligned")
+    K = int(w.size(-1))
+    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"w must have a multiple of 128 columns, got {K}")
+    codes = torch.empty((*w.shape[:-1], K // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((*w.shape[:-1], K // W4_GROUP), dtype=torch.uint8, device=w.device)
+    with torch.cuda.device(w.device):
+        capi.check(capi.load().moe_quantize_w4(_ptr(w), _DTYPES[w.dtype], w.numel() // W4_GROUP, _ptr(codes),
+                                               _ptr(scales), _stream(w.device)), "quantize_w4")
+    return codes, scales
+
+
+def _w4_shape(N: int, K: int) -> tuple:
+    return (-(-N // 16), -(-K // W4_CHUNK_K), W4_CHUNK_BYTES)
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """MXFP4 codes uint8 [N, K / 2] and scales uint8 [N, K / 32], or e of them [e, N, ...], in the MFMA operand layout:
+    uint8 [ceil(N / 16), ceil(K / 512), 4352], or [e, ...].  `out` (optional) receives them in place, e.g. one
+    expert's slot ``packed[e:e+1]`` of a larger buffer."""
+    _require_device("codes", codes)
+    _require_device("scales", scales, codes.device)
+    _check(codes.dtype == torch.uint8 and scales.dtype == torch.uint8, "codes and scales must be uint8")
+    _check(codes.dim() in (2, 3) and codes.is_contiguous() and scales.is_contiguous(),
+           "codes and scales must be [N, ...] or [e, N, ...] contiguous")
+    N, K = int(codes.size(-2)), 2 * int(codes.size(-1))
+    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"K must be a multiple of 128, got {K}")
+    _check(0 < N <= capi.MAX_W4_DIM, f"N must be in [1, {capi.MAX_W4_DIM}], got {N}")
+    _check(tuple(scales.shape) == (*codes.shape[:-1], K // W4_GROUP), "scales must be [..., N, K / 32] beside codes")
+    _check(codes.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "codes and scales must be 16-byte aligned")
+    n = int(codes.size(0)) if codes.dim() == 3 else 1
+    shape = (*codes.shape[:-2], *_w4_shape(N, K))
+    if out is None:
+        out = torch.empty(shape, dtype=torch.uint8, device=codes.device)
+    else:
+        _check(out.dtype == torch.uint8 and tuple(out.shape) == shape and out.is_contiguous(),
+               f"pack_w4 out must be uint8 {list(shape)} contiguous")
+        _require_device("pack_w4 out", out, codes.device)
+    with torch.cuda.device(codes.device):
+        capi.check(capi.load().moe_pack_w4(_ptr(codes), _ptr(scales), _ptr(out), n, N, K, _stream(codes.device)),
+                   "pack_w4")
+    return out
+
+
+def unpack_w4(packed: torch.Tensor, N: int, K: int):
+    """Inverse of pack_w4: (codes uint8 [.., N, K / 2], scales uint8 [.., N, K / 32])."""
+    _check_packed("packed", packed, N, K, batched=packed.dim() == 4)
+    lead = packed.shape[:-3]
+    codes = torch.empty((*lead, N, K // 2), dtype=torch.uint8, device=packed.device)
+    scales = torch.empty((*lead, N, K // W4_GROUP), dtype=torch.uint8, device=packed.device)
+    n = int(packed.size(0)) if packed.dim() == 4 else 1
+    with torch.cuda.device(packed.device):
+        capi.check(capi.load().moe_unpack_w4(_ptr(packed), _ptr(codes), _ptr(scales), n, N, K,
+                                             _stream(packed.device)), "unpack_w4")
+    return codes, scales
+
+
+def _check_packed(name, packed, N, K, batched, device=None):
+    _require_device(name, packed, device)
+    want = _w4_shape(N, K)
+    if packed.dtype != torch.uint8 or packed.dim() != 3 + batched or tuple(packed.shape[-3:]) != want \
+            or not packed.is_contiguous():
+        lead = "[e_local, " if batched else "["
+        raise RuntimeError(f"{name} must be a pack_w4 result uint8 {lead}{want[0]}, {want[1]}, {want[2]}] contiguous, "
+                           f"got {packed.dtype} {list(packed.shape)}")
+
+
+def _check_act(x, x_scale):
+    _require_device("x", x)
+    dev = x.device
+    _require_device("x_scale", x_scale, dev)
+    _check(x.dtype == torch.float8_e4m3fn and x.dim() == 2 and x.is_contiguous(), "x must be e4m3 [T, K] contiguous")
+    T, K = int(x.size(0)), int(x.size(1))
+    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"x must have a multiple of 128 columns, got {K}")
+    _check(T <= capi.MAX_T, f"T must be <= {capi.MAX_T}")
+    if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (K // 128, T) or not x_scale.is_contiguous():
+        raise RuntimeError(f"x_scale must be float32 [{K // 128}, {T}] contiguous")
+    return T, K, dev
+
+
+def linear_w4(x: torch.Tensor, x_scale: torch.Tensor, packed: torch.Tensor, n_out: int | None = None) -> torch.Tensor:
+    """bf16 [T, N] = x W^T for a dense layer in 4 bits: x and x_scale from quant_act (or router_quant), `packed` from
+    pack_w4.  `n_out` is N where it is not a multiple of 16."""
+    T, K, dev = _check_act(x, x_scale)
+    _check(packed.dim() == 3, "packed must be a pack_w4 result [row tiles, chunks, 4352]")
+    tiles = int(packed.size(0))
+    N = 16 * tiles if n_out is None else int(n_out)
+    if not 16 * (tiles - 1) < N <= 16 * tiles:
+        raise RuntimeError(f"n_out must be in [{16 * tiles - 15}, {16 * tiles}] for {tiles} packed row tiles, got {N}")
+    _check_packed("packed", packed, N, K, False, dev)
+    out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
+    with torch.cuda.device(dev):
+        capi.check(capi.load().moe_linear_w4(_ptr(x), _ptr(x_scale), _ptr(packed), T, N, K, _ptr(out), _stream(dev)),
+                   "linear_w4")
+    return out
+
+
+def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, ids: torch.Tensor,
+               weights: torch.Tensor, local_offset: int = 0) -> torch.Tensor:
+    """bf16 [T, hidden]: the routed experts of moe_forward with 4-bit weights, on the picks of any router.
+
+    x e4m3 [T, hidden] and x_scale as for linear_w4; w13 and w2 are pack_w4 results of [e_local, 2 * inter, hidden]
+    (rows [0, inter) multiply, SiLU takes rows [inter, 2 * inter), as in moe_forward) and [e_local, hidden, inter]; ids
+    int32 [T, top_k] and weights f32 [T, top_k] as route_topk gives them.  Picks outside [local_offset, local_offset +
+    e_local) are another rank's, or none, and add nothing; a token without local picks gets zeros.  hidden and inter
+    are multiples of 128."""
+    T, K, dev = _check_act(x, x_scale)
+    _check(w13.dim() == 4 and w2.dim() == 4, "w13 and w2 must be pack_w4 results [e_local, row tiles, chunks, 4352]")
+    E, inter = int(w13.size(0)), 8 * int(w13.size(1))
+    _check(inter % 128 == 0, "w13 must have 2 * inter rows, inter a multiple of 128")
+    _check_packed("w13", w13, 2 * inter, K, True, dev)
+    _check_packed("w2", w2, K, inter, True, dev)
+    _check(w2.size(0) == E, "w13 and w2 must have the same experts")
+    _check(ids.dim() == 2 and ids.dtype == torch.int32 and ids.size(0) == T and ids.is_contiguous(),
+           "ids must be int32 [T, top_k] contiguous")
+    _check(weights.dtype == torch.float32 and weights.shape == ids.shape and weights.is_contiguous(),
+           "weights must be float32 [T, top_k] contiguous")
+    _require_device("ids", ids, dev)
+    _require_device("weights", weights, dev)
+    k = int(ids.size(1))
+    lib = capi.load()
+    ws_bytes = int(lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k))
+    out = torch.empty((T, K), dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        capi.check(lib.moe_experts_w4(_ptr(x), _ptr(x_scale), _ptr(w13), _ptr(w2), _ptr(ids), _ptr(weights), T, K,
+                                      inter, E, k, int(local_offset), _ptr(ws), ws_bytes, _ptr(out), _stream(dev)),
+                   "experts_w4")
+    return out
+
+
 # --------------------------------------------------------------------------- inspection
 def workspace_views(ws: torch.Tensor, T: int, E: int) -> dict:
     """Typed views of the MOE_WS_* buffers inside a forward/route workspace.

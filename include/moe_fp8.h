@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define MOE_ABI_VERSION 2
+#define MOE_ABI_VERSION 3
 
 #define MOE_OK 0
 #define MOE_ERR_INVALID_ARG 1 /* bad size, null or misaligned pointer */
@@ -175,6 +175,87 @@ int moe_unpack_router(const void* router_packed, void* router_w_bf16, void* stre
 size_t moe_router_workspace_bytes(int T);
 int moe_router_quant(const void* hidden_bf16, const void* router_packed, int T, void* workspace,
                      size_t workspace_bytes, float* logits, void* hidden_fp8, float* hidden_scale, void* stream);
+
+/*
+ * General expert router (the layer's own fixed one is part of moe_forward):
+ *   s = sigmoid(logits) or softmax(logits)    exponentials in 64 bits, rounded to 32
+ *   v = s + bias                              bias f32 [n_experts] or NULL
+ *   kept groups: the topk_group of the n_group equal groups with the largest
+ *     sum of their group_top (1 or 2) largest v; ties to the lower group
+ *   ids     int32 [T, top_k]  the top_k largest v of the kept groups, ascending;
+ *                             ties to the lower expert
+ *   weights f32   [T, top_k]  s / (sum of the picks' s + 1e-20) * scale with
+ *                             renormalize, else s * scale
+ * logits [T, n_experts] of type dtype (enum moe_dtype), rows row_stride
+ * elements apart.  Experts whose logit or v is -inf or NaN are never picked; slots
+ * without a pick hold id -1, weight 0, last in the row.
+ * T <= MOE_MAX_ROUTE_T, n_experts <= MOE_MAX_EXPERTS, top_k <= MOE_MAX_TOP_K, n_group <=
+ * 64, top_k <= the kept groups' experts.
+ *
+ * moe_route_topk_backward: grad_logits [T, n_experts] of type dtype, contiguous, from
+ * grad_weights f32 [T, top_k] and the picks (ids outside [0, n_experts) count as
+ * none); the bias takes no gradient.
+ */
+enum moe_dtype { MOE_DTYPE_F32 = 0, MOE_DTYPE_BF16 = 1, MOE_DTYPE_F16 = 2 };
+enum moe_scoring { MOE_SCORING_SIGMOID = 0, MOE_SCORING_SOFTMAX = 1 };
+#define MOE_MAX_EXPERTS 1024
+#define MOE_MAX_TOP_K 64
+#define MOE_MAX_ROUTE_T (1 << 24)
+int moe_route_topk(const void* logits, int dtype, size_t row_stride, const float* bias, int T, int n_experts,
+                   int top_k, int scoring, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                   float* weights, int32_t* ids, void* stream);
+int moe_route_topk_backward(const float* grad_weights, const void* logits, int dtype, size_t row_stride,
+                            const int32_t* ids, int T, int n_experts, int top_k, int scoring, int renormalize,
+                            float scale, void* grad_logits, void* stream);
+
+/*
+ * Activations to block-scaled e4m3, the quantisation of moe_router_quant alone:
+ * x [T, K] of type dtype, rows row_stride elements (a multiple of 16 bytes) apart,
+ * K a multiple of 128 -> codes e4m3 [T, K], scale f32 [K / 128, T].
+ */
+int moe_quant_act(const void* x, int dtype, size_t row_stride, int T, int K, void* codes, float* scale, void* stream);
+
+/*
+ * 4-bit weights in OCP MXFP4: codes [N, K / 2] (two e2m1 elements a byte, the
+ * lower index in the low half), scales e8m0 [N, K / 32] (255: NaN).  K is a
+ * multiple of 128, N any, both at most MOE_MAX_W4_DIM.
+ *   moe_quantize_w4  groups x 32 contiguous elements of type dtype -> their codes
+ *                    and scales (a group with an infinity or NaN: scale 255);
+ *                    at most MOE_MAX_W4_GROUPS in one call
+ *   moe_pack_w4      n matrices -> the operand layout of the products,
+ *                    n * moe_packed_w4_bytes(N, K) bytes, at most 2^36 in one
+ *                    call; moe_unpack_w4 inverts it
+ *   moe_linear_w4    out bf16 [T, N] = x W^T; x e4m3 [T, K], x_scale f32 [K / 128, T]
+ */
+#define MOE_MAX_W4_DIM 262144
+#define MOE_MAX_W4_GROUPS ((size_t)1 << 29)
+int moe_quantize_w4(const void* w, int dtype, size_t groups, void* codes, void* scales, void* stream);
+size_t moe_packed_w4_bytes(int N, int K);
+int moe_pack_w4(const void* codes, const void* scales, void* packed, int n, int N, int K, void* stream);
+int moe_unpack_w4(const void* packed, void* codes, void* scales, int n, int N, int K, void* stream);
+int moe_linear_w4(const void* x, const float* x_scale, const void* packed, int T, int N, int K, void* out_bf16,
+                  void* stream);
+
+/*
+ * The routed experts' products with 4-bit weights, on picks of any router:
+ *   c = (W13[:I] x) * silu(W13[I:] x), requantised to e4m3 per 128 columns,
+ *   out[t] = sum over the token's local picks, in their order, of weight * W2 c
+ *   x         e4m3 [T, hidden]      x_scale f32 [hidden / 128, T]
+ *   w13       moe_pack_w4 of e_local matrices [2 * inter, hidden]
+ *   w2        moe_pack_w4 of e_local matrices [hidden, inter]
+ *   ids       int32 [T, top_k]; picks outside [offset, offset + e_local) are other
+ *             ranks' (or none) and add nothing
+ *   weights   f32 [T, top_k]
+ *   out_bf16  bf16 [T, hidden]
+ * hidden and inter are multiples of 128, e_local <= MOE_MAX_EXPERTS, top_k <=
+ * MOE_MAX_TOP_K, T <= MOE_MAX_T.  Pointers 16-byte aligned (ids and weights
+ * 4-byte); the workspace is the caller's (moe_experts_w4_workspace_bytes; 0 for sizes that are
+ * not accepted) and belongs to one call at a time.
+ */
+size_t moe_experts_w4_workspace_bytes(int T, int hidden, int inter, int e_local, int top_k);
+int moe_experts_w4(const void* x, const float* x_scale, const void* w13_packed, const void* w2_packed,
+                   const int32_t* ids, const float* weights, int T, int hidden, int inter, int e_local, int top_k,
+                   int local_expert_offset, void* workspace, size_t workspace_bytes, void* out_bf16, void* stream);
 
 #ifdef __cplusplus
 }
