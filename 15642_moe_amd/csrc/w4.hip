@@ -300,6 +300,21 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 
 __device__ __forceinline__ int chunk_begin(int KC, int wave, int waves) { return KC * wave / waves; }
 
+// Four outputs of row t from column n on.
+__device__ __forceinline__ void store_linear(uint16_t* __restrict__ out, int t, int n, int N, const v4f& y) {
+  if (n >= N) return;
+  uint16_t* dst = out + (size_t)t * N + n;
+  const uint32_t lo = bf16_pair(y[0], y[1]), hi = bf16_pair(y[2], y[3]);
+  if ((N & 3) == 0) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+  } else {
+    dst[0] = (uint16_t)lo;
+    if (n + 1 < N) dst[1] = (uint16_t)(lo >> 16);
+    if (n + 2 < N) dst[2] = (uint16_t)hi;
+    if (n + 3 < N) dst[3] = (uint16_t)(hi >> 16);
+  }
+}
+
 // y[t, n]: workgroup (row tiles nt*NT .., token group tg).
 template <int NT, int FR>
 __global__ void __launch_bounds__(512)
@@ -324,19 +339,176 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
   st.xs_stride = T;
   st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
   st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
-    const int t = t0 + 16 * f + (lane & 15), n = (n0 + p) * 16 + 4 * (lane >> 4);
-    if (t >= T || n >= N) return;
-    uint16_t* dst = out + (size_t)t * N + n;
-    const uint32_t lo = bf16_pair(y[0][0], y[0][1]), hi = bf16_pair(y[0][2], y[0][3]);
-    if ((N & 3) == 0) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-    } else {
-      dst[0] = (uint16_t)lo;
-      if (n + 1 < N) dst[1] = (uint16_t)(lo >> 16);
-      if (n + 2 < N) dst[2] = (uint16_t)hi;
-      if (n + 3 < N) dst[3] = (uint16_t)(hi >> 16);
-    }
+    const int t = t0 + 16 * f + (lane & 15);
+    if (t < T) store_linear(out, t, (n0 + p) * 16 + 4 * (lane >> 4), N, y[0]);
   });
+}
+
+// ---------------------------------------------------------------------------
+// Tiles, for many activation rows.  A workgroup of 8 waves multiplies 256 weight
+// rows with up to 32 * NC activation rows: wave (rw, cw) takes weight tiles 4 rw ..
+// + 4 and the fragments cw NC .. + NC of 16 activation rows.  The weights go from
+// global memory to the registers of the wave that owns their rows, three K-blocks
+// ahead (each of the two waves with the same rows loads them: the second load hits
+// L1); the activations, which every wave needs, go through LDS, a K-block ahead.  Per
+// K-block a wave reads 2 KB of LDS for each four MFMAs (128 clocks of its SIMD):
+// half of the LDS bandwidth with two waves a SIMD.
+//
+// LDS rows are 128 bytes; the 16-byte piece q of row m lies at position q ^ (m & 7),
+// so that eight lanes with eight consecutive rows read eight different banks' groups.
+// ---------------------------------------------------------------------------
+constexpr int TILE_THREADS = 512, TILE_ROWS = 256, TILE_MAX_NC = 4;
+constexpr int TILE_MAX_M = 32 * TILE_MAX_NC;  // activation rows
+struct TileLds {
+  uint8_t x[2][TILE_MAX_M * BLK];
+  float xs[2][TILE_MAX_M];
+  float amax[4][TILE_MAX_M];
+};
+__device__ __forceinline__ uint32_t tile_slot(int row, int piece) {
+  return (uint32_t)(row * BLK + ((piece ^ (row & 7)) << 4));
+}
+
+// acc[n][c]: the wave's 16 x 16 results.  row_of(m) -> {activation row, scale row}
+// pointers of tile row m < 32 NC.
+template <int NC, class RowOf>
+__device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&w)[4], int KB, size_t xs_stride,
+                                             RowOf&& row_of, v4f (&acc)[4][NC]) {
+  constexpr int M = 32 * NC, PIECES = M * 8, PER = (PIECES + TILE_THREADS - 1) / TILE_THREADS, NR = W4_CHUNK_BLOCKS;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
+  const uint8_t* src[PER];
+  uint32_t dst[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int q = tid + i * TILE_THREADS, m = q >> 3;
+    src[i] = row_of(m < M ? m : 0).first + (q & 7) * 16;
+    dst[i] = tile_slot(m, q & 7);
+  }
+  const float* scale = row_of(tid < M ? tid : 0).second;
+  u32x4 st[PER];
+  float ss;
+  auto fetch = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (PIECES % TILE_THREADS == 0 || tid + i * TILE_THREADS < PIECES)
+        st[i] = *reinterpret_cast<const u32x4*>(src[i] + (size_t)kb * BLK);
+    if (tid < M) ss = scale[(size_t)kb * xs_stride];
+  };
+  auto stage = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (PIECES % TILE_THREADS == 0 || tid + i * TILE_THREADS < PIECES)
+        *reinterpret_cast<u32x4*>(s.x[buf] + dst[i]) = st[i];
+    if (tid < M) s.xs[buf][tid] = ss;
+  };
+  u32x4 a[NR][4];
+  int sc[4], sc_next[4];
+  const int last = (KB - 1) / W4_CHUNK_BLOCKS;
+  auto load_a = [&](int chunk, auto bc) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      a[b][n] = *reinterpret_cast<const u32x4*>(w[n] + (size_t)chunk * W4_CHUNK_BYTES + (uint32_t)(b * W4_BLOCK_BYTES + lane * 16));
+  };
+  auto load_sc = [&](int chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      sc_next[n] = *reinterpret_cast<const int*>(w[n] + (size_t)chunk * W4_CHUNK_BYTES +
+                                                 (uint32_t)(W4_CHUNK_BLOCKS * W4_BLOCK_BYTES + lane * 4));
+  };
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[n][c] = zero4;
+
+  fetch(0);
+  load_sc(0);
+  load_a(0, std::integral_constant<int, 0>{});
+  load_a(0, std::integral_constant<int, 1>{});
+  load_a(0, std::integral_constant<int, 2>{});
+  stage(0);
+  __syncthreads();
+  const int i16 = lane & 15, g = lane >> 4;
+  for (int chunk = 0; chunk <= last; ++chunk) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sc[n] = sc_next[n];
+    static_for<NR>([&](auto bc) __attribute__((always_inline)) {
+      constexpr int b = decltype(bc)::value;
+      const int kb = chunk * NR + b;
+      if (kb >= KB) return;  // uniform
+      const bool more = kb + 1 < KB;
+      if (more) fetch(kb + 1);
+      // K-block kb + 3, into the slot that the last step used
+      load_a(b == 0 ? chunk : min(chunk + 1, last), std::integral_constant<int, (b + 3) % NR>{});
+      if constexpr (b == 0) load_sc(min(chunk + 1, last));
+      const uint8_t* xb = s.x[b & 1];
+      const float* xsb = s.xs[b & 1];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int m = (cw * NC + c) * 16 + i16;
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(xb + tile_slot(m, g));
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(xb + tile_slot(m, g + 4));
+        const float sx = xsb[m];
+        const v8i x = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n][c] += mfma_w4<b>(a[b][n], x, sc[n], zero4) * sx;
+      }
+      if (more) stage((b + 1) & 1);
+      __syncthreads();
+    });
+  }
+}
+
+// This workgroup's item of base .. n_work - 1, or -1.  They are cut into one run per XCD
+// (workgroup b runs on XCD b % XCDS), so the items that share a route tile's
+// activations share an L2.
+__device__ __forceinline__ int xcd_item(int base, int n_work) {
+  const int n = min(n_work - base, (int)gridDim.x), per = (n + XCDS - 1) / XCDS;
+  const int q = blockIdx.x / XCDS, i = (int)(blockIdx.x % XCDS) * per + q;
+  return q < per && i < n ? base + i : -1;
+}
+// Launches for `items` items at most, each below 2^32 threads: f(grid, first item).
+template <class F>
+void by_grids(size_t items, F&& f) {
+  for (size_t at = 0; at < items; at += MAX_GRID) {
+    const size_t n = items - at < MAX_GRID ? items - at : MAX_GRID;
+    f((unsigned)((n + XCDS - 1) / XCDS * XCDS), (int)at);
+  }
+}
+
+struct TileRow {
+  const uint8_t* first;
+  const float* second;
+};
+
+template <int NC>
+__global__ void __launch_bounds__(TILE_THREADS)
+linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs, const uint8_t* __restrict__ packed,
+                      int T, int N, int K, int base, uint16_t* __restrict__ out) {
+  __shared__ __align__(16) TileLds s;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int KC = w4_chunks(K), tiles = w4_tiles(N), blocks = (tiles + 15) / 16;
+  const int item = xcd_item(base, blocks * ((T + 32 * NC - 1) / (32 * NC)));
+  if (item < 0) return;
+  const int nb = item % blocks, t0 = item / blocks * (32 * NC);
+  const uint8_t* w[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    w[n] = packed + (size_t)min(nb * 16 + rw * 4 + n, tiles - 1) * KC * W4_CHUNK_BYTES;
+  v4f acc[4][NC];
+  tile_product<NC>(s, w, K / BLK, T, [&](int m) {
+    const int t = min(t0 + m, T - 1);  // padding rows reread the last one
+    return TileRow{x + (size_t)t * K, xs + t};
+  }, acc);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int t = t0 + (cw * NC + c) * 16 + (lane & 15);
+    if (t >= T) continue;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) store_linear(out, t, (nb * 16 + rw * 4 + n) * 16 + 4 * (lane >> 4), N, acc[n][c]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -350,12 +522,13 @@ struct Routes {
   int32_t* offsets;      // [e_local + 1] first route of each expert; the last: their number
   int32_t* n_tiles;      // [1]
   int4* tiles;           // {expert, first route, routes, 0}
-  int32_t* route_pick;   // [T k]
+  int32_t* route_pick;   // [T k] pick of each route; bit 31: its token's only local one
   int32_t* pick_route;   // [T k], -1 for picks of other experts
   int32_t* chunk_counts; // [chunks][e_local]
 };
 constexpr int SORT_THREADS = 1024, SORT_CHUNK = 8192;  // picks per workgroup
 constexpr int MAX_EXPERTS = 1024;
+constexpr int ONLY_BIT = (int)0x80000000u, PICK_MASK = 0x7FFFFFFF;
 
 // s_scan[0 .. n) exclusive prefix sums of v over the threads; returns this
 // thread's, `total` the sum.
@@ -379,8 +552,9 @@ __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
   return base + inc - v;
 }
 
-// Offsets and the tile list from expert `threadIdx.x`'s count; s_off / s_tp
-// [e_local] receive the first routes and tiles.
+// Offsets and the tile list from expert `threadIdx.x`'s count: an expert's
+// fragments of 16 routes, dealt evenly over as few tiles of at most bm routes as hold
+// them.
 __device__ __forceinline__ void publish_tiles(int cnt, int e_local, int bm, const Routes& r, int* s_off, int* s_tp,
                                               int* s_cnt, int* s_wave) {
   const int e = threadIdx.x;
@@ -399,56 +573,71 @@ __device__ __forceinline__ void publish_tiles(int cnt, int e_local, int bm, cons
   }
   __syncthreads();
   for (int i = e; i < tiles; i += SORT_THREADS) {
-    int lo = 0, hi = e_local - 1;  // the last expert whose first tile is at most i (and which has any)
+    int lo = 0, hi = e_local - 1;  // the last expert whose first tile is at most i: the one that has it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (s_tp[mid] <= i) lo = mid;
       else hi = mid - 1;
     }
-    const int m0 = (i - s_tp[lo]) * bm;
-    r.tiles[i] = make_int4(lo, s_off[lo] + m0, min(bm, s_cnt[lo] - m0), 0);
+    const int n = s_cnt[lo], nt = (n + bm - 1) / bm;
+    const int per = (((n + 15) >> 4) + nt - 1) / nt * 16, m0 = (i - s_tp[lo]) * per;
+    r.tiles[i] = make_int4(lo, s_off[lo] + m0, min(per, n - m0), 0);
+  }
+}
+
+// Local expert of a pick, or -1.
+__device__ __forceinline__ int local_expert(int id, int e_local, int offset) {
+  const int e = id - offset;
+  return id >= 0 && e >= 0 && e < e_local ? e : -1;
+}
+
+// Picks p0 .. p1 - 1 into their expert's places, from s_pos[e] on.
+__device__ __forceinline__ void place_picks(const int32_t* __restrict__ ids, int p0, int p1, int k, int e_local,
+                                            int offset, int* s_pos, const Routes& r) {
+  for (int p = p0 + (int)threadIdx.x; p < p1; p += SORT_THREADS) {
+    const int e = local_expert(ids[p], e_local, offset);
+    int at = -1;
+    if (e >= 0) {
+      int n = 0;
+      for (int j = p / k * k, j1 = j + k; j < j1; ++j) n += local_expert(ids[j], e_local, offset) >= 0 ? 1 : 0;
+      at = atomicAdd(&s_pos[e], 1);
+      r.route_pick[at] = p | (n == 1 ? ONLY_BIT : 0);
+    }
+    r.pick_route[p] = at;
+  }
+}
+__device__ __forceinline__ void count_picks(const int32_t* __restrict__ ids, int p0, int p1, int e_local, int offset,
+                                            int* s_cnt) {
+  for (int p = p0 + (int)threadIdx.x; p < p1; p += SORT_THREADS) {
+    const int e = local_expert(ids[p], e_local, offset);
+    if (e >= 0) atomicAdd(&s_cnt[e], 1);
   }
 }
 
 // All picks by one workgroup.
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_small_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, int bm, Routes r) {
+sort_small_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, int bm, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_pos[MAX_EXPERTS], s_wave[16];
   const int tid = threadIdx.x;
   s_pos[tid] = 0;
   __syncthreads();
-  for (int p = tid; p < picks; p += SORT_THREADS) {
-    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
-    if (e < (unsigned)e_local && ids[p] >= 0) atomicAdd(&s_pos[e], 1);
-  }
+  count_picks(ids, 0, picks, e_local, offset, s_pos);
   __syncthreads();
   publish_tiles(tid < e_local ? s_pos[tid] : 0, e_local, bm, r, s_off, s_tp, s_cnt, s_wave);
   __syncthreads();
   s_pos[tid] = tid < e_local ? s_off[tid] : 0;
   __syncthreads();
-  for (int p = tid; p < picks; p += SORT_THREADS) {
-    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
-    int at = -1;
-    if (e < (unsigned)e_local && ids[p] >= 0) {
-      at = atomicAdd(&s_pos[e], 1);
-      r.route_pick[at] = p;
-    }
-    r.pick_route[p] = at;
-  }
+  place_picks(ids, 0, picks, k, e_local, offset, s_pos, r);
 }
 
 // The same over several workgroups: counts of each SORT_CHUNK picks, ...
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_count_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, p0 = blockIdx.x * SORT_CHUNK;
   s_cnt[tid] = 0;
   __syncthreads();
-  const int p1 = min(picks, ((int)blockIdx.x + 1) * SORT_CHUNK);
-  for (int p = blockIdx.x * SORT_CHUNK + tid; p < p1; p += SORT_THREADS) {
-    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
-    if (e < (unsigned)e_local && ids[p] >= 0) atomicAdd(&s_cnt[e], 1);
-  }
+  count_picks(ids, p0, min(picks, p0 + SORT_CHUNK), e_local, offset, s_cnt);
   __syncthreads();
   if (tid < e_local) r.chunk_counts[(size_t)blockIdx.x * e_local + tid] = s_cnt[tid];
 }
@@ -473,21 +662,12 @@ sort_scan_kernel(int chunks, int e_local, int bm, Routes r) {
 }
 // ... and the places.
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_place_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, Routes r) {
+sort_place_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, Routes r) {
   __shared__ int s_pos[MAX_EXPERTS];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, p0 = blockIdx.x * SORT_CHUNK;
   if (tid < e_local) s_pos[tid] = r.chunk_counts[(size_t)blockIdx.x * e_local + tid];
   __syncthreads();
-  const int p1 = min(picks, ((int)blockIdx.x + 1) * SORT_CHUNK);
-  for (int p = blockIdx.x * SORT_CHUNK + tid; p < p1; p += SORT_THREADS) {
-    const unsigned e = (unsigned)ids[p] - (unsigned)offset;
-    int at = -1;
-    if (e < (unsigned)e_local && ids[p] >= 0) {
-      at = atomicAdd(&s_pos[e], 1);
-      r.route_pick[at] = p;
-    }
-    r.pick_route[p] = at;
-  }
+  place_picks(ids, p0, min(picks, p0 + SORT_CHUNK), k, e_local, offset, s_pos, r);
 }
 
 // GEMM1 and SwiGLU of (route tile, NP pairs of 16 gate and 16 up rows): rows
@@ -513,7 +693,7 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
     }
 #pragma unroll
     for (int f = 0; f < FR; ++f) {
-      const int t = r.route_pick[tile.y + min(16 * f + (lane & 15), tile.z - 1)] / a.k;
+      const int t = (r.route_pick[tile.y + min(16 * f + (lane & 15), tile.z - 1)] & PICK_MASK) / a.k;
       st.x[f] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
       st.xs[f] = a.xs + t;
     }
@@ -530,6 +710,19 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
       *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + (j * NP + p) * 16 + 4 * (lane >> 4)) = c;
     });
   }
+}
+
+// Four columns of a route's W2 c, times its weight: to Y, or to the output row of a
+// token that has no other local pick.
+__device__ __forceinline__ void store_y(const ExpertsW4& a, const Routes& r, float* __restrict__ Y, int route, int col,
+                                        const v4f& v) {
+  const int rp = r.route_pick[route], pick = rp & PICK_MASK;
+  const v4f y = v * a.weights[pick];
+  if (rp < 0)  // 0 + y, as the combine's sum of one: -0 becomes +0
+    *reinterpret_cast<uint2*>(a.out + (size_t)(pick / a.k) * a.H + col) =
+        make_uint2(bf16_pair(y[0] + 0.0f, y[1] + 0.0f), bf16_pair(y[2] + 0.0f, y[3] + 0.0f));
+  else
+    *reinterpret_cast<float4*>(Y + (size_t)route * a.H + col) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
 // GEMM2 of (route tile, NT 16-row tiles of W2), times the pick's weight.
@@ -561,19 +754,133 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
     st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
       const int m = 16 * f + (lane & 15);
       if (m >= tile.z) return;
-      const float w = a.weights[r.route_pick[tile.y + m]];
-      *reinterpret_cast<float4*>(Y + (size_t)(tile.y + m) * a.H + (j * NT + p) * 16 + 4 * (lane >> 4)) =
-          make_float4(y[0][0] * w, y[0][1] * w, y[0][2] * w, y[0][3] * w);
+      store_y(a, r, Y, tile.y + m, (j * NT + p) * 16 + 4 * (lane >> 4), y[0]);
     });
   }
 }
 
-// out[t] = the sum of its local picks' Y rows, in the order of the picks.
+// The experts' products in tiles (launched with route tiles of TILE_MAX_M).  f(NC) for
+// the fewest fragments that hold `rows`.
+template <int NC = 1, class F>
+__device__ __forceinline__ void by_rows(int rows, F&& f) {
+  if constexpr (NC < TILE_MAX_NC) {
+    if (rows > 32 * NC) return by_rows<NC + 1>(rows, f);
+  }
+  f(std::integral_constant<int, NC>{});
+}
+
+// GEMM1, SwiGLU and the FP8 requantisation of (route tile, 128 columns of the
+// intermediate): wave rw's weight tiles are 32 gate and the same 32 up rows.
+__global__ void __launch_bounds__(TILE_THREADS)
+experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__ Cq, float* __restrict__ Cs) {
+  __shared__ __align__(16) TileLds s;
+  const int IB = a.I / BLK;
+  const int item = xcd_item(base, *r.n_tiles * IB);
+  if (item < 0) return;
+  const int nb = item % IB;
+  const int4 tile = r.tiles[item / IB];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int KC = w4_chunks(a.H), tiles = 2 * a.I / 16;
+  const uint8_t* w[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int row = nb * 8 + 2 * rw + (n & 1) + (n >> 1) * (a.I / 16);
+    w[n] = a.w13 + ((size_t)tile.x * tiles + row) * KC * W4_CHUNK_BYTES;
+  }
+  by_rows(tile.z, [&](auto ncc) __attribute__((always_inline)) {
+    constexpr int NC = decltype(ncc)::value;
+    v4f acc[4][NC];
+    tile_product<NC>(s, w, a.H / BLK, a.T, [&](int m) {
+      const int t = (r.route_pick[tile.y + min(m, tile.z - 1)] & PICK_MASK) / a.k;
+      return TileRow{a.x + (size_t)t * a.H, a.xs + t};
+    }, acc);
+    // c in place of the gate's results, and the waves' largest magnitudes per route.
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float up = acc[2 + p][c][v];
+          acc[p][c][v] *= up / (1.0f + __expf(-up));
+          mx = fmaxf(mx, fabsf(acc[p][c][v]));
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      if (g == 0) s.amax[rw][(cw * NC + c) * 16 + lane] = mx;
+    }
+    __syncthreads();
+    uint8_t* codes = s.x[0];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int m = (cw * NC + c) * 16 + (lane & 15);
+      const float sc = fmaxf(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])) / E4M3_MAX, 1.0e-8f);
+      auto q = [&](float x) {
+        const float v = x / sc;
+        return v > E4M3_MAX ? E4M3_MAX : v < -E4M3_MAX ? -E4M3_MAX : v;
+      };
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        *reinterpret_cast<uint32_t*>(codes + tile_slot(m, 2 * rw + p) + 4 * g) =
+            cvt4_e4m3(q(acc[p][c][0]), q(acc[p][c][1]), q(acc[p][c][2]), q(acc[p][c][3]));
+      if (rw == 0 && g == 0 && m < tile.z) Cs[(size_t)(tile.y + m) * IB + nb] = sc;
+    }
+    __syncthreads();
+    for (int i = tid; i < tile.z * 8; i += TILE_THREADS)
+      *reinterpret_cast<u32x4*>(Cq + (size_t)(tile.y + (i >> 3)) * a.I + nb * BLK + (i & 7) * 16) =
+          *reinterpret_cast<const u32x4*>(codes + tile_slot(i >> 3, i & 7));
+  });
+}
+
+// GEMM2 of (route tile, 256 columns of the output; the last block may have 128).
+__global__ void __launch_bounds__(TILE_THREADS)
+experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __restrict__ Cq,
+                          const float* __restrict__ Cs, float* __restrict__ Y) {
+  __shared__ __align__(16) TileLds s;
+  const int tiles = a.H / 16, blocks = (tiles + 15) / 16, KB = a.I / BLK;
+  const int item = xcd_item(base, *r.n_tiles * blocks);
+  if (item < 0) return;
+  const int nb = item % blocks;
+  const int4 tile = r.tiles[item / blocks];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int KC = w4_chunks(a.I);
+  const uint8_t* w[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    w[n] = a.w2 + ((size_t)tile.x * tiles + min(nb * 16 + rw * 4 + n, tiles - 1)) * KC * W4_CHUNK_BYTES;
+  by_rows(tile.z, [&](auto ncc) __attribute__((always_inline)) {
+    constexpr int NC = decltype(ncc)::value;
+    v4f acc[4][NC];
+    tile_product<NC>(s, w, KB, 1, [&](int m) {
+      const size_t row = tile.y + min(m, tile.z - 1);
+      return TileRow{Cq + row * a.I, Cs + row * KB};
+    }, acc);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int m = (cw * NC + c) * 16 + (lane & 15);
+      if (m >= tile.z) continue;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int row = nb * 16 + rw * 4 + n;
+        if (row < tiles) store_y(a, r, Y, tile.y + m, row * 16 + 4 * (lane >> 4), acc[n][c]);
+      }
+    }
+  });
+}
+
+// out[t] = the sum of its local picks' Y rows, in the order of the picks, where it
+// has not just one.
 __global__ void __launch_bounds__(256)
 experts_combine_kernel(const float* __restrict__ Y, const int32_t* __restrict__ pick_route, int H, int k,
                        uint16_t* __restrict__ out) {
   const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= H) return;
+  int n = 0;
+  for (int j = 0; j < k; ++j) n += pick_route[(size_t)t * k + j] >= 0 ? 1 : 0;
+  if (n == 1) return;  // GEMM2 has written it
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int j = 0; j < k; ++j) {
     const int r = pick_route[(size_t)t * k + j];
@@ -645,10 +952,38 @@ hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, 
   return hipGetLastError();
 }
 
+// Fragments per wave of a tile launch: the fewest whole rounds of workgroups over
+// the CUs, each as long as its fragments and a constant share (weights, barriers).
+static int linear_tile_nc(int T, int tiles, int cus) {
+  int best = 1;
+  float least = 0.0f;
+  for (int nc = 1; nc <= TILE_MAX_NC; ++nc) {
+    const long long items = (long long)((tiles + 15) / 16) * ((T + 32 * nc - 1) / (32 * nc));
+    const float cost = (float)((items + cus - 1) / cus) * (nc + 1.5f);
+    if (nc == 1 || cost < least) { best = nc; least = cost; }
+  }
+  return best;
+}
+
 hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* packed, int T, int N, int K,
                             uint16_t* out, hipStream_t stream) {
   const int tiles = w4_tiles(N), KC = w4_chunks(K);
   const int waves = KC < 8 ? KC : 8;
+  if (T > 64) {
+    auto tile = [&](auto kernel, int nc) {
+      const size_t items = (size_t)((tiles + 15) / 16) * ((T + 32 * nc - 1) / (32 * nc));
+      by_grids(items, [&](unsigned grid, int base) {
+        kernel<<<grid, TILE_THREADS, 0, stream>>>(x, xs, packed, T, N, K, base, out);
+      });
+    };
+    switch (linear_tile_nc(T, tiles, device_cus())) {
+      case 1: tile(linear_w4_tile_kernel<1>, 1); break;
+      case 2: tile(linear_w4_tile_kernel<2>, 2); break;
+      case 3: tile(linear_w4_tile_kernel<3>, 3); break;
+      default: tile(linear_w4_tile_kernel<4>, 4); break;
+    }
+    return hipGetLastError();
+  }
   auto launch = [&](auto kernel, int nt, int fr) {
     const dim3 grid((tiles + nt - 1) / nt, (T + 16 * fr - 1) / (16 * fr));
     kernel<<<grid, 64 * waves, waves > 1 ? waves * nt * fr * 1024 : 0, stream>>>(x, xs, packed, T, N, K, out);
@@ -672,17 +1007,18 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   float* Cs = reinterpret_cast<float*>(ws + l.cs);
   float* Y = reinterpret_cast<float*>(ws + l.y);
   const int picks = a.T * a.k;
-  const int fr = a.T <= 16 ? 1 : 2, bm = 16 * fr;
+  const bool tile = a.T > 256;
+  const int fr = a.T <= 16 ? 1 : 2, bm = tile ? TILE_MAX_M : 16 * fr;
   hipError_t err;
   if (picks <= SORT_CHUNK) {
-    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, bm, r);
+    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, bm, r);
   } else {
     const int chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
     sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
     sort_scan_kernel<<<1, SORT_THREADS, 0, stream>>>(chunks, a.e_local, bm, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
+    sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, r);
   }
   if ((err = hipGetLastError()) != hipSuccess) return err;
   const size_t bound = max_tiles(picks, a.e_local, bm);
@@ -691,6 +1027,18 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
     const size_t fit = MAX_GRID / slices > 0 ? MAX_GRID / slices : 1;
     return (unsigned)((bound < fit ? bound : fit) * slices);
   };
+  if (tile) {
+    by_grids(bound * (a.I / BLK), [&](unsigned grid, int base) {
+      experts_gemm1_tile_kernel<<<grid, TILE_THREADS, 0, stream>>>(a, r, base, Cq, Cs);
+    });
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    by_grids(bound * ((a.H / 16 + 15) / 16), [&](unsigned grid, int base) {
+      experts_gemm2_tile_kernel<<<grid, TILE_THREADS, 0, stream>>>(a, r, base, Cq, Cs, Y);
+    });
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    experts_combine_kernel<<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, stream>>>(Y, r.pick_route, a.H, a.k, a.out);
+    return hipGetLastError();
+  }
   auto waves_of = [](int K) { return w4_chunks(K) < 8 ? w4_chunks(K) : 8; };
   {
     const int w = waves_of(a.H);

@@ -243,45 +243,64 @@ def moe_forward(hidden, hidden_scale, W13_packed, W13_scale, W2_packed, W2_scale
 
 
 # --------------------------------------------------------------------------- general router
+# A call of these operators may take the GPU 3 us, so the host's share counts: with one C call on plain integers, the
+# device switched only where another one is current, and the stream read as a raw handle, route_topk takes the
+# host 9 us at T = 1 where wrapped pointers, the device and stream objects took 14.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(what: str, fn, dev: torch.device, *args) -> None:
+    """fn(*args, stream) with `dev` current, on its current stream; RuntimeError for a non-zero status."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        capi.check(rc, what)
+
+
 _DTYPES = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}
 
 
-def _rows(name: str, x: torch.Tensor) -> int:
-    """Checks a [T, n] float input and returns its row stride in elements."""
+def _rows(name: str, x: torch.Tensor) -> tuple:
+    """Checks a [T, n] float input and returns T, n and its row stride in elements."""
     _require_device(name, x)
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
-    _check(x.dim() == 2, f"{name} must be two-dimensional")
-    _check(x.stride(1) == 1 or x.size(1) == 1, f"{name} must be contiguous along its last dimension")
-    return int(x.stride(0)) if x.size(0) > 1 else int(x.size(1))
+    if x.dim() != 2:
+        raise RuntimeError(f"{name} must be two-dimensional")
+    T, n = x.shape
+    stride, step = x.stride()
+    if step != 1 and n != 1:
+        raise RuntimeError(f"{name} must be contiguous along its last dimension")
+    return T, n, stride if T > 1 else n
 
 
 def _check_router(logits, top_k, scoring):
-    stride = _rows("logits", logits)
-    E = int(logits.size(1))
+    T, E, stride = _rows("logits", logits)
     if scoring not in capi.SCORING:
         raise RuntimeError(f"scoring must be one of {sorted(capi.SCORING)}, got {scoring!r}")
     if not 1 <= E <= capi.MAX_EXPERTS:
         raise RuntimeError(f"logits must have 1 to {capi.MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(capi.MAX_TOP_K, E):
         raise RuntimeError(f"top_k must be in [1, {min(capi.MAX_TOP_K, E)}], got {top_k}")
-    return int(logits.size(0)), E, stride
+    return T, E, stride
 
 
 def _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale):
     T, E, stride = _check_router(logits, top_k, scoring)
     dev = logits.device
     if bias is not None:
-        _check(bias.dtype == torch.float32 and bias.dim() == 1 and bias.numel() == E and bias.is_contiguous(),
-               f"bias must be float32 [{E}] contiguous")
+        if bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous():
+            raise RuntimeError(f"bias must be float32 [{E}] contiguous")
         _require_device("bias", bias, dev)
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        capi.check(capi.load().moe_route_topk(
-            _ptr(logits), _DTYPES[logits.dtype], stride, _ptr(bias) if bias is not None else None, T, E, top_k,
-            capi.SCORING[scoring], n_group, topk_group, group_top, int(renormalize), scale, _ptr(weights), _ptr(ids),
-            _stream(dev)), "route_topk")
+    _call("route_topk", capi.load().moe_route_topk, dev, logits.data_ptr(), _DTYPES[logits.dtype], stride,
+          None if bias is None else bias.data_ptr(), T, E, top_k, capi.SCORING[scoring], n_group, topk_group, group_top,
+          renormalize, scale, weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -299,10 +318,9 @@ def route_topk_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: t
     _require_device("ids", ids, dev)
     _require_device("grad_weights", grad_weights, dev)
     out = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
-        capi.check(capi.load().moe_route_topk_backward(
-            _ptr(grad_weights), _ptr(logits), _DTYPES[logits.dtype], stride, _ptr(ids), T, E, top_k,
-            capi.SCORING[scoring], int(renormalize), float(scale), _ptr(out), _stream(dev)), "route_topk_backward")
+    _call("route_topk_backward", capi.load().moe_route_topk_backward, dev, grad_weights.data_ptr(), logits.data_ptr(),
+          _DTYPES[logits.dtype], stride, ids.data_ptr(), T, E, top_k, capi.SCORING[scoring], renormalize, scale,
+          out.data_ptr())
     return out
 
 
@@ -336,10 +354,10 @@ def route_topk(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, scor
     id -1 and weight 0.  The weights are differentiable in the logits; the bias only balances load and takes no
     gradient.  `experts_w4` takes the result as it is."""
     topk_group = n_group if topk_group is None else topk_group
-    form = (int(top_k), scoring, int(n_group), int(topk_group), int(group_top), bool(renormalize), float(scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteTopK.apply(logits, None if bias is None else bias.detach(), *form)
-    return _route_topk(logits, bias, *form)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouteTopK.apply(logits, None if bias is None else bias.detach(), top_k, scoring, n_group, topk_group,
+                                group_top, renormalize, scale)
+    return _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale)
 
 
 # --------------------------------------------------------------------------- 4-bit weights
@@ -348,19 +366,23 @@ W4_CHUNK_BYTES = 4352    # 16 rows x 512 elements of K, codes and scales
 W4_CHUNK_K = 512
 
 
+def _check_size(T: int, K: int) -> None:
+    if not 0 < K <= capi.MAX_W4_DIM or K % 128:
+        raise RuntimeError(f"x must have a multiple of 128 columns, got {K}")
+    if T > capi.MAX_T:
+        raise RuntimeError(f"T must be <= {capi.MAX_T}")
+
+
 def quant_act(x: torch.Tensor):
     """[T, K] float32, bfloat16 or float16 (K a multiple of 128) -> (e4m3 [T, K], scale f32 [K / 128, T]): the
     quantisation that router_quant does on its way, for the input of linear_w4 and experts_w4 or moe_forward."""
-    stride = _rows("x", x)
-    T, K = int(x.size(0)), int(x.size(1))
-    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"x must have a multiple of 128 columns, got {K}")
-    _check(T <= capi.MAX_T, f"T must be <= {capi.MAX_T}")
+    T, K, stride = _rows("x", x)
+    _check_size(T, K)
     _check(stride * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0, "x must have 16-byte aligned rows")
     codes = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty((K // 128, T), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        capi.check(capi.load().moe_quant_act(_ptr(x), _DTYPES[x.dtype], stride, T, K, _ptr(codes), _ptr(scale),
-                                             _stream(x.device)), "quant_act")
+    _call("quant_act", capi.load().moe_quant_act, x.device, x.data_ptr(), _DTYPES[x.dtype], stride, T, K,
+          codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -376,9 +398,8 @@ def quantize_w4(w: torch.Tensor):
     _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"w must have a multiple of 128 columns, got {K}")
     codes = torch.empty((*w.shape[:-1], K // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((*w.shape[:-1], K // W4_GROUP), dtype=torch.uint8, device=w.device)
-    with torch.cuda.device(w.device):
-        capi.check(capi.load().moe_quantize_w4(_ptr(w), _DTYPES[w.dtype], w.numel() // W4_GROUP, _ptr(codes),
-                                               _ptr(scales), _stream(w.device)), "quantize_w4")
+    _call("quantize_w4", capi.load().moe_quantize_w4, w.device, w.data_ptr(), _DTYPES[w.dtype], w.numel() // W4_GROUP,
+          codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -408,9 +429,7 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None 
         _check(out.dtype == torch.uint8 and tuple(out.shape) == shape and out.is_contiguous(),
                f"pack_w4 out must be uint8 {list(shape)} contiguous")
         _require_device("pack_w4 out", out, codes.device)
-    with torch.cuda.device(codes.device):
-        capi.check(capi.load().moe_pack_w4(_ptr(codes), _ptr(scales), _ptr(out), n, N, K, _stream(codes.device)),
-                   "pack_w4")
+    _call("pack_w4", capi.load().moe_pack_w4, codes.device, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, N, K)
     return out
 
 
@@ -421,16 +440,15 @@ def unpack_w4(packed: torch.Tensor, N: int, K: int):
     codes = torch.empty((*lead, N, K // 2), dtype=torch.uint8, device=packed.device)
     scales = torch.empty((*lead, N, K // W4_GROUP), dtype=torch.uint8, device=packed.device)
     n = int(packed.size(0)) if packed.dim() == 4 else 1
-    with torch.cuda.device(packed.device):
-        capi.check(capi.load().moe_unpack_w4(_ptr(packed), _ptr(codes), _ptr(scales), n, N, K,
-                                             _stream(packed.device)), "unpack_w4")
+    _call("unpack_w4", capi.load().moe_unpack_w4, packed.device, packed.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+          n, N, K)
     return codes, scales
 
 
 def _check_packed(name, packed, N, K, batched, device=None):
     _require_device(name, packed, device)
     want = _w4_shape(N, K)
-    if packed.dtype != torch.uint8 or packed.dim() != 3 + batched or tuple(packed.shape[-3:]) != want \
+    if packed.dtype != torch.uint8 or packed.dim() != 3 + batched or packed.shape[-3:] != want \
             or not packed.is_contiguous():
         lead = "[e_local, " if batched else "["
         raise RuntimeError(f"{name} must be a pack_w4 result uint8 {lead}{want[0]}, {want[1]}, {want[2]}] contiguous, "
@@ -442,10 +460,9 @@ def _check_act(x, x_scale):
     dev = x.device
     _require_device("x_scale", x_scale, dev)
     _check(x.dtype == torch.float8_e4m3fn and x.dim() == 2 and x.is_contiguous(), "x must be e4m3 [T, K] contiguous")
-    T, K = int(x.size(0)), int(x.size(1))
-    _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"x must have a multiple of 128 columns, got {K}")
-    _check(T <= capi.MAX_T, f"T must be <= {capi.MAX_T}")
-    if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (K // 128, T) or not x_scale.is_contiguous():
+    T, K = x.shape
+    _check_size(T, K)
+    if x_scale.dtype != torch.float32 or x_scale.shape != (K // 128, T) or not x_scale.is_contiguous():
         raise RuntimeError(f"x_scale must be float32 [{K // 128}, {T}] contiguous")
     return T, K, dev
 
@@ -461,9 +478,8 @@ def linear_w4(x: torch.Tensor, x_scale: torch.Tensor, packed: torch.Tensor, n_ou
         raise RuntimeError(f"n_out must be in [{16 * tiles - 15}, {16 * tiles}] for {tiles} packed row tiles, got {N}")
     _check_packed("packed", packed, N, K, False, dev)
     out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
-        capi.check(capi.load().moe_linear_w4(_ptr(x), _ptr(x_scale), _ptr(packed), T, N, K, _ptr(out), _stream(dev)),
-                   "linear_w4")
+    _call("linear_w4", capi.load().moe_linear_w4, dev, x.data_ptr(), x_scale.data_ptr(), packed.data_ptr(), T, N, K,
+          out.data_ptr())
     return out
 
 
@@ -494,10 +510,8 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     ws_bytes = int(lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k))
     out = torch.empty((T, K), dtype=torch.bfloat16, device=dev)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        capi.check(lib.moe_experts_w4(_ptr(x), _ptr(x_scale), _ptr(w13), _ptr(w2), _ptr(ids), _ptr(weights), T, K,
-                                      inter, E, k, int(local_offset), _ptr(ws), ws_bytes, _ptr(out), _stream(dev)),
-                   "experts_w4")
+    _call("experts_w4", lib.moe_experts_w4, dev, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+          ids.data_ptr(), weights.data_ptr(), T, K, inter, E, k, local_offset, ws.data_ptr(), ws_bytes, out.data_ptr())
     return out
 
 
