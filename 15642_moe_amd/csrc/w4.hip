@@ -345,66 +345,68 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 }
 
 // ---------------------------------------------------------------------------
-// Tiles, for many activation rows.  A workgroup of 8 waves multiplies 256 weight
-// rows with up to 32 * NC activation rows: wave (rw, cw) takes weight tiles 4 rw ..
-// + 4 and the fragments cw NC .. + NC of 16 activation rows.  The weights go from
-// global memory to the registers of the wave that owns their rows, three K-blocks
-// ahead (each of the two waves with the same rows loads them: the second load hits
-// L1); the activations, which every wave needs, go through LDS, a K-block ahead.  Per
-// K-block a wave reads 2 KB of LDS for each four MFMAs (128 clocks of its SIMD):
-// half of the LDS bandwidth with two waves a SIMD.
+// Tiles, for many activation rows.  A workgroup of 4 waves multiplies 256 weight
+// rows with up to 64 activation rows, two workgroups a CU: a wave takes 4 weight tiles
+// and all the rows.  The weights go from global memory to the registers of the wave
+// that owns their rows, three K-blocks ahead; the activations, which every wave
+// needs, go through LDS, a chunk of four K-blocks ahead.  Per K-block a wave reads 2 KB
+// of LDS for each four MFMAs (128 clocks of its SIMD): half of the LDS bandwidth with
+// two waves a SIMD.
 //
 // LDS rows are 128 bytes; the 16-byte piece q of row m lies at position q ^ (m & 7),
 // so that eight lanes with eight consecutive rows read eight different banks' groups.
 // ---------------------------------------------------------------------------
-constexpr int TILE_THREADS = 512, TILE_ROWS = 256, TILE_MAX_NC = 4;
-constexpr int TILE_MAX_M = 32 * TILE_MAX_NC;  // activation rows
+constexpr int TILE_THREADS = 256, TILE_MAX_NC = 4;
+constexpr int TILE_MAX_M = 16 * TILE_MAX_NC;  // activation rows
 struct TileLds {
-  uint8_t x[2][TILE_MAX_M * BLK];
-  float xs[2][TILE_MAX_M];
+  uint8_t x[2][W4_CHUNK_BLOCKS * TILE_MAX_M * BLK];  // [K-block][row][128]
+  float xs[2][W4_CHUNK_BLOCKS * TILE_MAX_M];
+  size_t row[TILE_MAX_M];  // byte offset of each activation row
   float amax[4][TILE_MAX_M];
 };
 __device__ __forceinline__ uint32_t tile_slot(int row, int piece) {
   return (uint32_t)(row * BLK + ((piece ^ (row & 7)) << 4));
 }
 
-// acc[n][c]: the wave's 16 x 16 results.  row_of(m) -> {activation row, scale row}
-// pointers of tile row m < 32 NC.
+// acc[n][c]: the wave's 16 x 16 results.  row_of(m): the activation row of tile row
+// m < 16 NC, of `K` bytes at x, its scales at xs + row * xs_row + kb * xs_block.
 template <int NC, class RowOf>
-__device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&w)[4], int KB, size_t xs_stride,
-                                             RowOf&& row_of, v4f (&acc)[4][NC]) {
-  constexpr int M = 32 * NC, PIECES = M * 8, PER = (PIECES + TILE_THREADS - 1) / TILE_THREADS, NR = W4_CHUNK_BLOCKS;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+__device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&w)[4], int K, const uint8_t* x,
+                                             const float* xs, size_t xs_row, size_t xs_block, RowOf&& row_of,
+                                             v4f (&acc)[4][NC]) {
+  constexpr int M = 16 * NC, NR = W4_CHUNK_BLOCKS, PER = M * NR * 8 / TILE_THREADS;  // 16-byte pieces per thread
+  const int tid = threadIdx.x, lane = tid & 63, KB = K / BLK, last = (KB - 1) / NR;
   const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
-  const uint8_t* src[PER];
-  uint32_t dst[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int q = tid + i * TILE_THREADS, m = q >> 3;
-    src[i] = row_of(m < M ? m : 0).first + (q & 7) * 16;
-    dst[i] = tile_slot(m, q & 7);
-  }
-  const float* scale = row_of(tid < M ? tid : 0).second;
+  // Thread tid fetches piece tid % 32 of the chunk's 512 bytes of rows tid / 32 + 16 i,
+  // and the scale of row tid % M, K-block tid / M.
+  const int piece = tid & 31;
+  const float* scale = xs + (size_t)row_of(tid % M) * xs_row + (size_t)(tid / M) * xs_block;
+  if (tid < M) s.row[tid] = (size_t)row_of(tid) * K;
+  __syncthreads();
   u32x4 st[PER];
-  float ss;
-  auto fetch = [&](int kb) __attribute__((always_inline)) {
+  float ss = 0.0f;
+  auto fetch = [&](int chunk) __attribute__((always_inline)) {
+    const int kb = chunk * NR + (piece >> 3);
+    const uint8_t* src = x + (size_t)(kb < KB ? kb : 0) * BLK + (piece & 7) * 16;  // past the end: zeros
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (PIECES % TILE_THREADS == 0 || tid + i * TILE_THREADS < PIECES)
-        st[i] = *reinterpret_cast<const u32x4*>(src[i] + (size_t)kb * BLK);
-    if (tid < M) ss = scale[(size_t)kb * xs_stride];
+      st[i] = *reinterpret_cast<const u32x4*>(src + s.row[(tid >> 5) + i * (TILE_THREADS / 32)]);
+    ss = tid < M * NR && chunk * NR + tid / M < KB ? scale[(size_t)chunk * NR * xs_block] : 0.0f;
   };
-  auto stage = [&](int buf) __attribute__((always_inline)) {
+  auto stage = [&](int chunk) __attribute__((always_inline)) {
+    const int buf = chunk & 1;
+    if (chunk * NR + (piece >> 3) >= KB) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) st[i] = u32x4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (PIECES % TILE_THREADS == 0 || tid + i * TILE_THREADS < PIECES)
-        *reinterpret_cast<u32x4*>(s.x[buf] + dst[i]) = st[i];
-    if (tid < M) s.xs[buf][tid] = ss;
+      *reinterpret_cast<u32x4*>(s.x[buf] + (piece >> 3) * (M * BLK) +
+                                tile_slot((tid >> 5) + i * (TILE_THREADS / 32), piece & 7)) = st[i];
+    if (tid < M * NR) s.xs[buf][tid] = ss;
   };
   u32x4 a[NR][4];
   int sc[4], sc_next[4];
-  const int last = (KB - 1) / W4_CHUNK_BLOCKS;
   auto load_a = [&](int chunk, auto bc) __attribute__((always_inline)) {
     constexpr int b = decltype(bc)::value;
 #pragma unroll
@@ -430,33 +432,43 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   stage(0);
   __syncthreads();
   const int i16 = lane & 15, g = lane >> 4;
+#pragma unroll 1
   for (int chunk = 0; chunk <= last; ++chunk) {
+    const int buf = chunk & 1;
+    const uint8_t* xb = s.x[buf];
+    const float* xsb = s.xs[buf];
 #pragma unroll
     for (int n = 0; n < 4; ++n) sc[n] = sc_next[n];
-    static_for<NR>([&](auto bc) __attribute__((always_inline)) {
-      constexpr int b = decltype(bc)::value;
-      const int kb = chunk * NR + b;
-      if (kb >= KB) return;  // uniform
-      const bool more = kb + 1 < KB;
-      if (more) fetch(kb + 1);
-      // K-block kb + 3, into the slot that the last step used
-      load_a(b == 0 ? chunk : min(chunk + 1, last), std::integral_constant<int, (b + 3) % NR>{});
-      if constexpr (b == 0) load_sc(min(chunk + 1, last));
-      const uint8_t* xb = s.x[b & 1];
-      const float* xsb = s.xs[b & 1];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int m = (cw * NC + c) * 16 + i16;
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(xb + tile_slot(m, g));
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(xb + tile_slot(m, g + 4));
-        const float sx = xsb[m];
-        const v8i x = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int n = 0; n < 4; ++n) acc[n][c] += mfma_w4<b>(a[b][n], x, sc[n], zero4) * sx;
+    if (chunk < last) fetch(chunk + 1);
+    // Fragment j of the chunk: K-block j / NC, rows 16 (j % NC) ..; its LDS reads run one
+    // fragment ahead of its MFMAs.
+    u32x4 lo[2], hi[2];
+    float sx[2];
+    auto read = [&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value, bb = j / NC, m0 = j % NC * 16;
+      lo[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g));
+      hi[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g + 4));
+      sx[j & 1] = xsb[bb * M + m0 + i16];
+    };
+    read(std::integral_constant<int, 0>{});
+    static_for<NR * NC>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value, bb = j / NC, c = j % NC;
+      if constexpr (c == 0) {  // K-block bb + 3, into the slot that the last one used
+        load_a(bb == 0 ? chunk : min(chunk + 1, last), std::integral_constant<int, (bb + 3) % NR>{});
+        if constexpr (bb == 0) load_sc(min(chunk + 1, last));
       }
-      if (more) stage((b + 1) & 1);
-      __syncthreads();
+      if constexpr (j + 1 < NR * NC) read(std::integral_constant<int, j + 1>{});
+      const v8i xv = __builtin_bit_cast(v8i, __builtin_shufflevector(lo[j & 1], hi[j & 1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        acc[n][c] += mfma_w4<bb>(a[bb][n], xv, sc[n], zero4) * sx[j & 1];
+        // Keeps the addition here: the compiler would sink it to the loop's end, with the
+        // products of the whole chunk in registers until then.
+        __asm__ volatile("" : "+v"(acc[n][c]));
+      }
     });
+    if (chunk < last) stage(chunk + 1);
+    __syncthreads();
   }
 }
 
@@ -477,34 +489,27 @@ void by_grids(size_t items, F&& f) {
   }
 }
 
-struct TileRow {
-  const uint8_t* first;
-  const float* second;
-};
-
 template <int NC>
-__global__ void __launch_bounds__(TILE_THREADS)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
 linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs, const uint8_t* __restrict__ packed,
                       int T, int N, int K, int base, uint16_t* __restrict__ out) {
   __shared__ __align__(16) TileLds s;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(K), tiles = w4_tiles(N), blocks = (tiles + 15) / 16;
-  const int item = xcd_item(base, blocks * ((T + 32 * NC - 1) / (32 * NC)));
+  const int item = xcd_item(base, blocks * ((T + 16 * NC - 1) / (16 * NC)));
   if (item < 0) return;
-  const int nb = item % blocks, t0 = item / blocks * (32 * NC);
+  const int nb = item % blocks, t0 = item / blocks * (16 * NC);
   const uint8_t* w[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n)
     w[n] = packed + (size_t)min(nb * 16 + rw * 4 + n, tiles - 1) * KC * W4_CHUNK_BYTES;
   v4f acc[4][NC];
-  tile_product<NC>(s, w, K / BLK, T, [&](int m) {
-    const int t = min(t0 + m, T - 1);  // padding rows reread the last one
-    return TileRow{x + (size_t)t * K, xs + t};
-  }, acc);
+  // Padding rows reread the last one.
+  tile_product<NC>(s, w, K, x, xs, 1, T, [&](int m) { return min(t0 + m, T - 1); }, acc);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int t = t0 + (cw * NC + c) * 16 + (lane & 15);
+    const int t = t0 + c * 16 + (lane & 15);
     if (t >= T) continue;
 #pragma unroll
     for (int n = 0; n < 4; ++n) store_linear(out, t, (nb * 16 + rw * 4 + n) * 16 + 4 * (lane >> 4), N, acc[n][c]);
@@ -764,14 +769,14 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
 template <int NC = 1, class F>
 __device__ __forceinline__ void by_rows(int rows, F&& f) {
   if constexpr (NC < TILE_MAX_NC) {
-    if (rows > 32 * NC) return by_rows<NC + 1>(rows, f);
+    if (rows > 16 * NC) return by_rows<NC + 1>(rows, f);
   }
   f(std::integral_constant<int, NC>{});
 }
 
 // GEMM1, SwiGLU and the FP8 requantisation of (route tile, 128 columns of the
 // intermediate): wave rw's weight tiles are 32 gate and the same 32 up rows.
-__global__ void __launch_bounds__(TILE_THREADS)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
 experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__ Cq, float* __restrict__ Cs) {
   __shared__ __align__(16) TileLds s;
   const int IB = a.I / BLK;
@@ -780,7 +785,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
   const int nb = item % IB;
   const int4 tile = r.tiles[item / IB];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(a.H), tiles = 2 * a.I / 16;
   const uint8_t* w[4];
 #pragma unroll
@@ -791,9 +796,8 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
   by_rows(tile.z, [&](auto ncc) __attribute__((always_inline)) {
     constexpr int NC = decltype(ncc)::value;
     v4f acc[4][NC];
-    tile_product<NC>(s, w, a.H / BLK, a.T, [&](int m) {
-      const int t = (r.route_pick[tile.y + min(m, tile.z - 1)] & PICK_MASK) / a.k;
-      return TileRow{a.x + (size_t)t * a.H, a.xs + t};
+    tile_product<NC>(s, w, a.H, a.x, a.xs, 1, a.T, [&](int m) {
+      return (r.route_pick[tile.y + min(m, tile.z - 1)] & PICK_MASK) / a.k;
     }, acc);
     // c in place of the gate's results, and the waves' largest magnitudes per route.
 #pragma unroll
@@ -809,13 +813,13 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
         }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (g == 0) s.amax[rw][(cw * NC + c) * 16 + lane] = mx;
+      if (g == 0) s.amax[rw][c * 16 + lane] = mx;
     }
     __syncthreads();
     uint8_t* codes = s.x[0];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = (cw * NC + c) * 16 + (lane & 15);
+      const int m = c * 16 + (lane & 15);
       const float sc = fmaxf(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])) / E4M3_MAX, 1.0e-8f);
       auto q = [&](float x) {
         const float v = x / sc;
@@ -835,7 +839,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
 }
 
 // GEMM2 of (route tile, 256 columns of the output; the last block may have 128).
-__global__ void __launch_bounds__(TILE_THREADS)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
 experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __restrict__ Cq,
                           const float* __restrict__ Cs, float* __restrict__ Y) {
   __shared__ __align__(16) TileLds s;
@@ -845,7 +849,7 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
   const int nb = item % blocks;
   const int4 tile = r.tiles[item / blocks];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(a.I);
   const uint8_t* w[4];
 #pragma unroll
@@ -854,13 +858,10 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
   by_rows(tile.z, [&](auto ncc) __attribute__((always_inline)) {
     constexpr int NC = decltype(ncc)::value;
     v4f acc[4][NC];
-    tile_product<NC>(s, w, KB, 1, [&](int m) {
-      const size_t row = tile.y + min(m, tile.z - 1);
-      return TileRow{Cq + row * a.I, Cs + row * KB};
-    }, acc);
+    tile_product<NC>(s, w, a.I, Cq, Cs, KB, 1, [&](int m) { return tile.y + min(m, tile.z - 1); }, acc);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = (cw * NC + c) * 16 + (lane & 15);
+      const int m = c * 16 + (lane & 15);
       if (m >= tile.z) continue;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -958,8 +959,8 @@ static int linear_tile_nc(int T, int tiles, int cus) {
   int best = 1;
   float least = 0.0f;
   for (int nc = 1; nc <= TILE_MAX_NC; ++nc) {
-    const long long items = (long long)((tiles + 15) / 16) * ((T + 32 * nc - 1) / (32 * nc));
-    const float cost = (float)((items + cus - 1) / cus) * (nc + 1.5f);
+    const long long items = (long long)((tiles + 15) / 16) * ((T + 16 * nc - 1) / (16 * nc));
+    const float cost = (float)((items + 2 * cus - 1) / (2 * cus)) * (nc + 1.5f);  // two workgroups a CU
     if (nc == 1 || cost < least) { best = nc; least = cost; }
   }
   return best;
@@ -971,7 +972,7 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
   const int waves = KC < 8 ? KC : 8;
   if (T > 64) {
     auto tile = [&](auto kernel, int nc) {
-      const size_t items = (size_t)((tiles + 15) / 16) * ((T + 32 * nc - 1) / (32 * nc));
+      const size_t items = (size_t)((tiles + 15) / 16) * ((T + 16 * nc - 1) / (16 * nc));
       by_grids(items, [&](unsigned grid, int base) {
         kernel<<<grid, TILE_THREADS, 0, stream>>>(x, xs, packed, T, N, K, base, out);
       });
