@@ -349,18 +349,19 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 // rows with up to 64 activation rows, two workgroups a CU: a wave takes 4 weight tiles
 // and all the rows.  The weights go from global memory to the registers of the wave
 // that owns their rows, three K-blocks ahead; the activations, which every wave
-// needs, go through LDS, a chunk of four K-blocks ahead.  Per K-block a wave reads 2 KB
+// needs, go through LDS, a step of two K-blocks ahead.  Per K-block a wave reads 2 KB
 // of LDS for each four MFMAs (128 clocks of its SIMD): half of the LDS bandwidth with
 // two waves a SIMD.
 //
 // LDS rows are 128 bytes; the 16-byte piece q of row m lies at position q ^ (m & 7),
 // so that eight lanes with eight consecutive rows read eight different banks' groups.
 // ---------------------------------------------------------------------------
-constexpr int TILE_THREADS = 256, TILE_MAX_NC = 4;
-constexpr int TILE_MAX_M = 16 * TILE_MAX_NC;  // activation rows
+constexpr int TILE_ROWS = 256, TILE_CW = 2, TILE_THREADS = 256 * TILE_CW, TILE_MAX_NC = 5;
+constexpr int TILE_COLS = 16 * TILE_CW, TILE_MAX_M = TILE_COLS * TILE_MAX_NC;  // activation rows
+constexpr int STEP_BLOCKS = 2;  // K-blocks of activations that are staged at once
 struct TileLds {
-  uint8_t x[2][W4_CHUNK_BLOCKS * TILE_MAX_M * BLK];  // [K-block][row][128]
-  float xs[2][W4_CHUNK_BLOCKS * TILE_MAX_M];
+  uint8_t x[2][STEP_BLOCKS * TILE_MAX_M * BLK];  // [K-block][row][128]
+  float xs[2][STEP_BLOCKS * TILE_MAX_M];
   size_t row[TILE_MAX_M];  // byte offset of each activation row
   float amax[4][TILE_MAX_M];
 };
@@ -374,36 +375,36 @@ template <int NC, class RowOf>
 __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&w)[4], int K, const uint8_t* x,
                                              const float* xs, size_t xs_row, size_t xs_block, RowOf&& row_of,
                                              v4f (&acc)[4][NC]) {
-  constexpr int M = 16 * NC, NR = W4_CHUNK_BLOCKS, PER = M * NR * 8 / TILE_THREADS;  // 16-byte pieces per thread
+  constexpr int M = TILE_COLS * NC, NR = W4_CHUNK_BLOCKS, NS = STEP_BLOCKS;
+  constexpr int PIECES = NS * 8, PER = M * PIECES / TILE_THREADS;  // 16-byte pieces of a row's step, and per thread
   const int tid = threadIdx.x, lane = tid & 63, KB = K / BLK, last = (KB - 1) / NR;
+  const int cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
-  // Thread tid fetches piece tid % 32 of the chunk's 512 bytes of rows tid / 32 + 16 i,
-  // and the scale of row tid % M, K-block tid / M.
-  const int piece = tid & 31;
+  // Thread tid fetches one piece of the step's K-blocks of rows tid / PIECES +
+  // (TILE_THREADS / PIECES) i, and the scale of row tid % M, K-block tid / M.
+  const int piece = tid % PIECES, row0 = tid / PIECES;
   const float* scale = xs + (size_t)row_of(tid % M) * xs_row + (size_t)(tid / M) * xs_block;
   if (tid < M) s.row[tid] = (size_t)row_of(tid) * K;
   __syncthreads();
   u32x4 st[PER];
   float ss = 0.0f;
-  auto fetch = [&](int chunk) __attribute__((always_inline)) {
-    const int kb = chunk * NR + (piece >> 3);
-    const uint8_t* src = x + (size_t)(kb < KB ? kb : 0) * BLK + (piece & 7) * 16;  // past the end: zeros
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      st[i] = *reinterpret_cast<const u32x4*>(src + s.row[(tid >> 5) + i * (TILE_THREADS / 32)]);
-    ss = tid < M * NR && chunk * NR + tid / M < KB ? scale[(size_t)chunk * NR * xs_block] : 0.0f;
+  // Piece i of a step: its load (past the end of K: anything), and its write to LDS
+  // (zeros there, which the padded weights need: a NaN code times zero is NaN).
+  auto fetch = [&](int step, int i) __attribute__((always_inline)) {
+    const int kb = step * NS + (piece >> 3);
+    st[i] = *reinterpret_cast<const u32x4*>(x + s.row[row0 + i * (TILE_THREADS / PIECES)] +
+                                            (size_t)(kb < KB ? kb : 0) * BLK + (piece & 7) * 16);
   };
-  auto stage = [&](int chunk) __attribute__((always_inline)) {
-    const int buf = chunk & 1;
-    if (chunk * NR + (piece >> 3) >= KB) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) st[i] = u32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      *reinterpret_cast<u32x4*>(s.x[buf] + (piece >> 3) * (M * BLK) +
-                                tile_slot((tid >> 5) + i * (TILE_THREADS / 32), piece & 7)) = st[i];
-    if (tid < M * NR) s.xs[buf][tid] = ss;
+  auto stage = [&](int step, int i) __attribute__((always_inline)) {
+    if (step * NS + (piece >> 3) >= KB) st[i] = u32x4{0, 0, 0, 0};
+    *reinterpret_cast<u32x4*>(s.x[step & 1] + (piece >> 3) * (M * BLK) +
+                              tile_slot(row0 + i * (TILE_THREADS / PIECES), piece & 7)) = st[i];
+  };
+  auto fetch_scale = [&](int step) __attribute__((always_inline)) {
+    ss = tid < M * NS && step * NS + tid / M < KB ? scale[(size_t)step * NS * xs_block] : 0.0f;
+  };
+  auto stage_scale = [&](int step) __attribute__((always_inline)) {
+    if (tid < M * NS) s.xs[step & 1][tid] = ss;
   };
   u32x4 a[NR][4];
   int sc[4], sc_next[4];
@@ -424,51 +425,68 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[n][c] = zero4;
 
-  fetch(0);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) fetch(0, i);
+  fetch_scale(0);
   load_sc(0);
   load_a(0, std::integral_constant<int, 0>{});
   load_a(0, std::integral_constant<int, 1>{});
   load_a(0, std::integral_constant<int, 2>{});
-  stage(0);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) stage(0, i);
+  stage_scale(0);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) fetch(1, i);
+  fetch_scale(1);
   __syncthreads();
-  const int i16 = lane & 15, g = lane >> 4;
+  const int i16 = cw * (16 * NC) + (lane & 15), g = lane >> 4;
 #pragma unroll 1
   for (int chunk = 0; chunk <= last; ++chunk) {
-    const int buf = chunk & 1;
-    const uint8_t* xb = s.x[buf];
-    const float* xsb = s.xs[buf];
 #pragma unroll
     for (int n = 0; n < 4; ++n) sc[n] = sc_next[n];
-    if (chunk < last) fetch(chunk + 1);
-    // Fragment j of the chunk: K-block j / NC, rows 16 (j % NC) ..; its LDS reads run one
-    // fragment ahead of its MFMAs.
-    u32x4 lo[2], hi[2];
-    float sx[2];
-    auto read = [&](auto jc) __attribute__((always_inline)) {
-      constexpr int j = decltype(jc)::value, bb = j / NC, m0 = j % NC * 16;
-      lo[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g));
-      hi[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g + 4));
-      sx[j & 1] = xsb[bb * M + m0 + i16];
-    };
-    read(std::integral_constant<int, 0>{});
-    static_for<NR * NC>([&](auto jc) __attribute__((always_inline)) {
-      constexpr int j = decltype(jc)::value, bb = j / NC, c = j % NC;
-      if constexpr (c == 0) {  // K-block bb + 3, into the slot that the last one used
-        load_a(bb == 0 ? chunk : min(chunk + 1, last), std::integral_constant<int, (bb + 3) % NR>{});
-        if constexpr (bb == 0) load_sc(min(chunk + 1, last));
-      }
-      if constexpr (j + 1 < NR * NC) read(std::integral_constant<int, j + 1>{});
-      const v8i xv = __builtin_bit_cast(v8i, __builtin_shufflevector(lo[j & 1], hi[j & 1], 0, 1, 2, 3, 4, 5, 6, 7));
+    static_for<NR / NS>([&](auto hc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value;
+      const int step = chunk * (NR / NS) + h;
+      const uint8_t* xb = s.x[h & 1];
+      const float* xsb = s.xs[h & 1];
+      // Fragment j of the step: K-block j / NC, rows 16 (j % NC) ..; its LDS reads run one
+      // fragment ahead of its MFMAs.  Between the first half of the fragments the next
+      // step's activations go to LDS (past the last: the buffer takes zeros), between
+      // the second those of the step after it come in.
+      u32x4 lo[2], hi[2];
+      float sx[2];
+      auto read = [&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value, bb = j / NC, m0 = j % NC * 16;
+        lo[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g));
+        hi[j & 1] = *reinterpret_cast<const u32x4*>(xb + bb * (M * BLK) + tile_slot(m0 + i16, g + 4));
+        sx[j & 1] = xsb[bb * M + m0 + i16];
+      };
+      read(std::integral_constant<int, 0>{});
+      static_for<NS * NC>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value, bb = h * NS + j / NC, c = j % NC;
+        if constexpr (c == 0) {  // K-block bb + 3, into the slot that the last one used
+          load_a(bb == 0 ? chunk : min(chunk + 1, last), std::integral_constant<int, (bb + 3) % NR>{});
+          if constexpr (bb == 0) load_sc(min(chunk + 1, last));
+        }
+        if constexpr (j + 1 < NS * NC) read(std::integral_constant<int, j + 1>{});
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of this fragment's MFMAs
+        const v8i xv = __builtin_bit_cast(v8i, __builtin_shufflevector(lo[j & 1], hi[j & 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        acc[n][c] += mfma_w4<bb>(a[bb][n], xv, sc[n], zero4) * sx[j & 1];
-        // Keeps the addition here: the compiler would sink it to the loop's end, with the
-        // products of the whole chunk in registers until then.
-        __asm__ volatile("" : "+v"(acc[n][c]));
-      }
+        for (int n = 0; n < 4; ++n) {
+          acc[n][c] += mfma_w4<bb>(a[bb][n], xv, sc[n], zero4) * sx[j & 1];
+          // Keeps the addition here: the compiler would sink it to the loop's end, with the
+          // products of the whole chunk in registers until then.
+          __asm__ volatile("" : "+v"(acc[n][c]));
+        }
+        if constexpr (j < PER) stage(step + 1, j);
+        if constexpr (j == PER - 1) {
+          stage_scale(step + 1);
+          fetch_scale(step + 2);
+        }
+        if constexpr (j >= PER) fetch(step + 2, j - PER);
+      });
+      __syncthreads();
     });
-    if (chunk < last) stage(chunk + 1);
-    __syncthreads();
   }
 }
 
@@ -495,11 +513,11 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
                       int T, int N, int K, int base, uint16_t* __restrict__ out) {
   __shared__ __align__(16) TileLds s;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(K), tiles = w4_tiles(N), blocks = (tiles + 15) / 16;
-  const int item = xcd_item(base, blocks * ((T + 16 * NC - 1) / (16 * NC)));
+  const int item = xcd_item(base, blocks * ((T + TILE_COLS * NC - 1) / (TILE_COLS * NC)));
   if (item < 0) return;
-  const int nb = item % blocks, t0 = item / blocks * (16 * NC);
+  const int nb = item % blocks, t0 = item / blocks * (TILE_COLS * NC);
   const uint8_t* w[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n)
@@ -507,12 +525,41 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
   v4f acc[4][NC];
   // Padding rows reread the last one.
   tile_product<NC>(s, w, K, x, xs, 1, T, [&](int m) { return min(t0 + m, T - 1); }, acc);
+  // The results in bf16 through LDS, [row][256] with the 16-byte pieces spread as the
+  // activations' are, so that 32 lanes store 512 contiguous bytes (straight from the
+  // registers, 8 bytes a lane, the stores took 8 of 37 us at T = 1501, N = 7168, K = 2048).
+  uint8_t* tile = s.x[0];
+  constexpr int HALF = TILE_COLS * NC / 2;  // rows that fit at a time: 512 bytes each
+  static_assert(HALF * 512 <= (int)sizeof(s.x), "half of the rows");
+  const int n0 = nb * TILE_ROWS;
+  for (int half = 0; half < 2; ++half) {
+    if (half > 0) __syncthreads();
+    if (cw == half) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int t = t0 + c * 16 + (lane & 15);
-    if (t >= T) continue;
+      for (int c = 0; c < NC; ++c) {
+        const int m = c * 16 + (lane & 15);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) store_linear(out, t, (nb * 16 + rw * 4 + n) * 16 + 4 * (lane >> 4), N, acc[n][c]);
+        for (int n = 0; n < 4; ++n) {
+          const int col = (rw * 4 + n) * 16 + 4 * (lane >> 4);  // of 256
+          *reinterpret_cast<uint2*>(tile + m * 512 + (((col >> 3) ^ (m & 7)) << 4) + (col & 4) * 2) =
+              make_uint2(bf16_pair(acc[n][c][0], acc[n][c][1]), bf16_pair(acc[n][c][2], acc[n][c][3]));
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < HALF * 32; i += TILE_THREADS) {
+      const int m = i >> 5, q = i & 31, t = t0 + half * HALF + m, n = n0 + q * 8;
+      if (t >= T || n >= N) continue;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + m * 512 + ((q ^ (m & 7)) << 4));
+      uint16_t* dst = out + (size_t)t * N + n;
+      if ((N & 7) == 0) {
+        *reinterpret_cast<u32x4*>(dst) = v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (n + k < N) dst[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+      }
+    }
   }
 }
 
@@ -557,14 +604,36 @@ __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
   return base + inc - v;
 }
 
+// Routes per tile at most.  A launch of the tile kernels takes whole rounds of its items
+// (tile, weight block) over the CUs, each about as long as its fragments of 32 routes and
+// 1.2 more (K = 7168, 1 to 5 of them: 28, 34, 44, 60, 71 us a round); of the sizes the one
+// with the shortest sum over GEMM1 (n1 weight blocks, k1 K-blocks) and GEMM2 is taken.
+struct TilePlan {
+  int bm;  // a fixed size, or 0: chosen
+  int n1, k1, n2, k2, cus;
+};
+
 // Offsets and the tile list from expert `threadIdx.x`'s count: an expert's
 // fragments of 16 routes, dealt evenly over as few tiles of at most bm routes as hold
 // them.
-__device__ __forceinline__ void publish_tiles(int cnt, int e_local, int bm, const Routes& r, int* s_off, int* s_tp,
-                                              int* s_cnt, int* s_wave) {
+__device__ __forceinline__ void publish_tiles(int cnt, int e_local, const TilePlan& plan, const Routes& r, int* s_off,
+                                              int* s_tp, int* s_cnt, int* s_wave) {
   const int e = threadIdx.x;
-  int total, tiles;
+  int total, tiles, bm = plan.bm;
   const int off = block_scan(cnt, s_wave, total);
+  if (bm == 0) {
+    float least = 0.0f;
+    for (int m = TILE_MAX_M; m >= 2 * TILE_COLS; m -= TILE_COLS) {
+      block_scan((cnt + m - 1) / m, s_wave, tiles);
+      const float item = (float)total / (float)(TILE_COLS * max(tiles, 1)) + 1.2f;
+      const float cost = item * ((float)((tiles * plan.n1 + plan.cus - 1) / plan.cus * plan.k1) +
+                                 (float)((tiles * plan.n2 + plan.cus - 1) / plan.cus * plan.k2));
+      if (m == TILE_MAX_M || cost < least) {
+        least = cost;
+        bm = m;
+      }
+    }
+  }
   const int tp = block_scan((cnt + bm - 1) / bm, s_wave, tiles);
   if (e < e_local) {
     s_off[e] = off;
@@ -621,14 +690,14 @@ __device__ __forceinline__ void count_picks(const int32_t* __restrict__ ids, int
 
 // All picks by one workgroup.
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_small_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, int bm, Routes r) {
+sort_small_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, TilePlan plan, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_pos[MAX_EXPERTS], s_wave[16];
   const int tid = threadIdx.x;
   s_pos[tid] = 0;
   __syncthreads();
   count_picks(ids, 0, picks, e_local, offset, s_pos);
   __syncthreads();
-  publish_tiles(tid < e_local ? s_pos[tid] : 0, e_local, bm, r, s_off, s_tp, s_cnt, s_wave);
+  publish_tiles(tid < e_local ? s_pos[tid] : 0, e_local, plan, r, s_off, s_tp, s_cnt, s_wave);
   __syncthreads();
   s_pos[tid] = tid < e_local ? s_off[tid] : 0;
   __syncthreads();
@@ -648,13 +717,13 @@ sort_count_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int o
 }
 // ... each chunk's first places, ...
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_scan_kernel(int chunks, int e_local, int bm, Routes r) {
+sort_scan_kernel(int chunks, int e_local, TilePlan plan, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_wave[16];
   const int e = threadIdx.x;
   int cnt = 0;
   if (e < e_local)
     for (int c = 0; c < chunks; ++c) cnt += r.chunk_counts[(size_t)c * e_local + e];
-  publish_tiles(cnt, e_local, bm, r, s_off, s_tp, s_cnt, s_wave);
+  publish_tiles(cnt, e_local, plan, r, s_off, s_tp, s_cnt, s_wave);
   if (e < e_local) {
     int at = s_off[e];
     for (int c = 0; c < chunks; ++c) {
@@ -769,7 +838,7 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
 template <int NC = 1, class F>
 __device__ __forceinline__ void by_rows(int rows, F&& f) {
   if constexpr (NC < TILE_MAX_NC) {
-    if (rows > 16 * NC) return by_rows<NC + 1>(rows, f);
+    if (rows > TILE_COLS * NC) return by_rows<NC + 1>(rows, f);
   }
   f(std::integral_constant<int, NC>{});
 }
@@ -785,7 +854,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
   const int nb = item % IB;
   const int4 tile = r.tiles[item / IB];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(a.H), tiles = 2 * a.I / 16;
   const uint8_t* w[4];
 #pragma unroll
@@ -813,13 +882,13 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
         }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (g == 0) s.amax[rw][c * 16 + lane] = mx;
+      if (g == 0) s.amax[rw][(cw * NC + c) * 16 + lane] = mx;
     }
     __syncthreads();
     uint8_t* codes = s.x[0];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = c * 16 + (lane & 15);
+      const int m = (cw * NC + c) * 16 + (lane & 15);
       const float sc = fmaxf(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])) / E4M3_MAX, 1.0e-8f);
       auto q = [&](float x) {
         const float v = x / sc;
@@ -849,7 +918,7 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
   const int nb = item % blocks;
   const int4 tile = r.tiles[item / blocks];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(a.I);
   const uint8_t* w[4];
 #pragma unroll
@@ -861,7 +930,7 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
     tile_product<NC>(s, w, a.I, Cq, Cs, KB, 1, [&](int m) { return tile.y + min(m, tile.z - 1); }, acc);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = c * 16 + (lane & 15);
+      const int m = (cw * NC + c) * 16 + (lane & 15);
       if (m >= tile.z) continue;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -959,8 +1028,8 @@ static int linear_tile_nc(int T, int tiles, int cus) {
   int best = 1;
   float least = 0.0f;
   for (int nc = 1; nc <= TILE_MAX_NC; ++nc) {
-    const long long items = (long long)((tiles + 15) / 16) * ((T + 16 * nc - 1) / (16 * nc));
-    const float cost = (float)((items + 2 * cus - 1) / (2 * cus)) * (nc + 1.5f);  // two workgroups a CU
+    const long long items = (long long)((tiles + 15) / 16) * ((T + TILE_COLS * nc - 1) / (TILE_COLS * nc));
+    const float cost = (float)((items + cus - 1) / cus) * (nc + 1.2f);
     if (nc == 1 || cost < least) { best = nc; least = cost; }
   }
   return best;
@@ -972,7 +1041,7 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
   const int waves = KC < 8 ? KC : 8;
   if (T > 64) {
     auto tile = [&](auto kernel, int nc) {
-      const size_t items = (size_t)((tiles + 15) / 16) * ((T + 16 * nc - 1) / (16 * nc));
+      const size_t items = (size_t)((tiles + 15) / 16) * ((T + TILE_COLS * nc - 1) / (TILE_COLS * nc));
       by_grids(items, [&](unsigned grid, int base) {
         kernel<<<grid, TILE_THREADS, 0, stream>>>(x, xs, packed, T, N, K, base, out);
       });
@@ -981,7 +1050,8 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
       case 1: tile(linear_w4_tile_kernel<1>, 1); break;
       case 2: tile(linear_w4_tile_kernel<2>, 2); break;
       case 3: tile(linear_w4_tile_kernel<3>, 3); break;
-      default: tile(linear_w4_tile_kernel<4>, 4); break;
+      case 4: tile(linear_w4_tile_kernel<4>, 4); break;
+      default: tile(linear_w4_tile_kernel<5>, 5); break;
     }
     return hipGetLastError();
   }
@@ -1009,20 +1079,21 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   float* Y = reinterpret_cast<float*>(ws + l.y);
   const int picks = a.T * a.k;
   const bool tile = a.T > 256;
-  const int fr = a.T <= 16 ? 1 : 2, bm = tile ? TILE_MAX_M : 16 * fr;
+  const int fr = a.T <= 16 ? 1 : 2;
+  const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus()};
   hipError_t err;
   if (picks <= SORT_CHUNK) {
-    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, bm, r);
+    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, plan, r);
   } else {
     const int chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
     sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    sort_scan_kernel<<<1, SORT_THREADS, 0, stream>>>(chunks, a.e_local, bm, r);
+    sort_scan_kernel<<<1, SORT_THREADS, 0, stream>>>(chunks, a.e_local, plan, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
     sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, r);
   }
   if ((err = hipGetLastError()) != hipSuccess) return err;
-  const size_t bound = max_tiles(picks, a.e_local, bm);
+  const size_t bound = max_tiles(picks, a.e_local, tile ? 2 * TILE_COLS : 16 * fr);
   // Workgroups: every tile's slices, or as many tiles' as fit, which then loop.
   auto grid_of = [&](int slices) {
     const size_t fit = MAX_GRID / slices > 0 ? MAX_GRID / slices : 1;
