@@ -356,14 +356,20 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 // LDS rows are 128 bytes; the 16-byte piece q of row m lies at position q ^ (m & 7),
 // so that eight lanes with eight consecutive rows read eight different banks' groups.
 // ---------------------------------------------------------------------------
-constexpr int TILE_ROWS = 256, TILE_CW = 2, TILE_THREADS = 256 * TILE_CW, TILE_MAX_NC = 5;
+constexpr int TILE_ROWS = 256, TILE_CW = 1, TILE_THREADS = 256 * TILE_CW, TILE_MAX_NC = 5;
 constexpr int TILE_COLS = 16 * TILE_CW, TILE_MAX_M = TILE_COLS * TILE_MAX_NC;  // activation rows
 constexpr int STEP_BLOCKS = 2;  // K-blocks of activations that are staged at once
 struct TileLds {
   uint8_t x[2][STEP_BLOCKS * TILE_MAX_M * BLK];  // [K-block][row][128]
   float xs[2][STEP_BLOCKS * TILE_MAX_M];
   size_t row[TILE_MAX_M];  // byte offset of each activation row
-  float amax[4][TILE_MAX_M];
+  union {
+    float amax[4][TILE_MAX_M];  // GEMM1
+    struct {                    // GEMM2
+      int token[TILE_MAX_M];
+      float weight[TILE_MAX_M];
+    };
+  };
 };
 __device__ __forceinline__ uint32_t tile_slot(int row, int piece) {
   return (uint32_t)(row * BLK + ((piece ^ (row & 7)) << 4));
@@ -385,7 +391,6 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   const int piece = tid % PIECES, row0 = tid / PIECES;
   const float* scale = xs + (size_t)row_of(tid % M) * xs_row + (size_t)(tid / M) * xs_block;
   if (tid < M) s.row[tid] = (size_t)row_of(tid) * K;
-  __syncthreads();
   u32x4 st[PER];
   float ss = 0.0f;
   // Piece i of a step: its load (past the end of K: anything), and its write to LDS
@@ -425,13 +430,14 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[n][c] = zero4;
 
-#pragma unroll
-  for (int i = 0; i < PER; ++i) fetch(0, i);
-  fetch_scale(0);
   load_sc(0);
   load_a(0, std::integral_constant<int, 0>{});
   load_a(0, std::integral_constant<int, 1>{});
   load_a(0, std::integral_constant<int, 2>{});
+  fetch_scale(0);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) fetch(0, i);
 #pragma unroll
   for (int i = 0; i < PER; ++i) stage(0, i);
   stage_scale(0);
@@ -529,10 +535,10 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
   // activations' are, so that 32 lanes store 512 contiguous bytes (straight from the
   // registers, 8 bytes a lane, the stores took 8 of 37 us at T = 1501, N = 7168, K = 2048).
   uint8_t* tile = s.x[0];
-  constexpr int HALF = TILE_COLS * NC / 2;  // rows that fit at a time: 512 bytes each
-  static_assert(HALF * 512 <= (int)sizeof(s.x), "half of the rows");
+  constexpr int HALF = 16 * NC;  // rows at a time, a wave column's: 512 bytes each
+  static_assert(HALF * 512 <= (int)sizeof(s.x), "a wave column's rows");
   const int n0 = nb * TILE_ROWS;
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < TILE_CW; ++half) {
     if (half > 0) __syncthreads();
     if (cw == half) {
 #pragma unroll
@@ -574,13 +580,21 @@ struct Routes {
   int32_t* offsets;      // [e_local + 1] first route of each expert; the last: their number
   int32_t* n_tiles;      // [1]
   int4* tiles;           // {expert, first route, routes, 0}
-  int32_t* route_pick;   // [T k] pick of each route; bit 31: its token's only local one
+  int32_t* route_token;  // [T k] token of each route; bit 31: its only local one
+  float* route_weight;   // [T k]
   int32_t* pick_route;   // [T k], -1 for picks of other experts
   int32_t* chunk_counts; // [chunks][e_local]
 };
-constexpr int SORT_THREADS = 1024, SORT_CHUNK = 8192;  // picks per workgroup
+// One workgroup sorts up to SORT_SMALL picks (its atomics on a few experts' counters take
+// 3 ns a pick); more are cut into at most SORT_MAX_CHUNKS chunks of at least
+// SORT_THREADS.
+constexpr int SORT_THREADS = 1024, SORT_SMALL = 2048, SORT_MAX_CHUNKS = 64;
+inline int sort_chunk(size_t picks) {
+  const size_t per = (picks + SORT_MAX_CHUNKS - 1) / SORT_MAX_CHUNKS;
+  return (int)((per + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
+}
 constexpr int MAX_EXPERTS = 1024;
-constexpr int ONLY_BIT = (int)0x80000000u, PICK_MASK = 0x7FFFFFFF;
+constexpr int ONLY_BIT = (int)0x80000000u, TOKEN_MASK = 0x7FFFFFFF;
 
 // s_scan[0 .. n) exclusive prefix sums of v over the threads; returns this
 // thread's, `total` the sum.
@@ -666,16 +680,18 @@ __device__ __forceinline__ int local_expert(int id, int e_local, int offset) {
 }
 
 // Picks p0 .. p1 - 1 into their expert's places, from s_pos[e] on.
-__device__ __forceinline__ void place_picks(const int32_t* __restrict__ ids, int p0, int p1, int k, int e_local,
+__device__ __forceinline__ void place_picks(const int32_t* __restrict__ ids, const float* __restrict__ weights, int p0, int p1, int k, int e_local,
                                             int offset, int* s_pos, const Routes& r) {
   for (int p = p0 + (int)threadIdx.x; p < p1; p += SORT_THREADS) {
     const int e = local_expert(ids[p], e_local, offset);
     int at = -1;
     if (e >= 0) {
+      const int t = p / k;
       int n = 0;
-      for (int j = p / k * k, j1 = j + k; j < j1; ++j) n += local_expert(ids[j], e_local, offset) >= 0 ? 1 : 0;
+      for (int j = t * k, j1 = j + k; j < j1; ++j) n += local_expert(ids[j], e_local, offset) >= 0 ? 1 : 0;
       at = atomicAdd(&s_pos[e], 1);
-      r.route_pick[at] = p | (n == 1 ? ONLY_BIT : 0);
+      r.route_token[at] = t | (n == 1 ? ONLY_BIT : 0);
+      r.route_weight[at] = weights[p];
     }
     r.pick_route[p] = at;
   }
@@ -690,7 +706,7 @@ __device__ __forceinline__ void count_picks(const int32_t* __restrict__ ids, int
 
 // All picks by one workgroup.
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_small_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, TilePlan plan, Routes r) {
+sort_small_kernel(const int32_t* __restrict__ ids, const float* __restrict__ weights, int picks, int k, int e_local, int offset, TilePlan plan, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_pos[MAX_EXPERTS], s_wave[16];
   const int tid = threadIdx.x;
   s_pos[tid] = 0;
@@ -701,47 +717,43 @@ sort_small_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local
   __syncthreads();
   s_pos[tid] = tid < e_local ? s_off[tid] : 0;
   __syncthreads();
-  place_picks(ids, 0, picks, k, e_local, offset, s_pos, r);
+  place_picks(ids, weights, 0, picks, k, e_local, offset, s_pos, r);
 }
 
-// The same over several workgroups: counts of each SORT_CHUNK picks, ...
+// The same over several workgroups, `chunk` picks each: their counts, ...
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_count_kernel(const int32_t* __restrict__ ids, int picks, int e_local, int offset, Routes r) {
+sort_count_kernel(const int32_t* __restrict__ ids, int picks, int chunk, int e_local, int offset, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS];
-  const int tid = threadIdx.x, p0 = blockIdx.x * SORT_CHUNK;
+  const int tid = threadIdx.x, p0 = blockIdx.x * chunk;
   s_cnt[tid] = 0;
   __syncthreads();
-  count_picks(ids, p0, min(picks, p0 + SORT_CHUNK), e_local, offset, s_cnt);
+  count_picks(ids, p0, min(picks, p0 + chunk), e_local, offset, s_cnt);
   __syncthreads();
   if (tid < e_local) r.chunk_counts[(size_t)blockIdx.x * e_local + tid] = s_cnt[tid];
 }
-// ... each chunk's first places, ...
+// The counts of expert `threadIdx.x` in chunks 0 .. n - 1 (at most SORT_MAX_CHUNKS).
+__device__ __forceinline__ int sum_chunks(const Routes& r, int n, int e_local) {
+  int sum = 0;
+#pragma unroll 8
+  for (int c = 0; c < n; ++c) sum += r.chunk_counts[(size_t)c * e_local + threadIdx.x];
+  return sum;
+}
+// ... the offsets and tiles from their sums, ...
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_scan_kernel(int chunks, int e_local, TilePlan plan, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_wave[16];
-  const int e = threadIdx.x;
-  int cnt = 0;
-  if (e < e_local)
-    for (int c = 0; c < chunks; ++c) cnt += r.chunk_counts[(size_t)c * e_local + e];
-  publish_tiles(cnt, e_local, plan, r, s_off, s_tp, s_cnt, s_wave);
-  if (e < e_local) {
-    int at = s_off[e];
-    for (int c = 0; c < chunks; ++c) {
-      const size_t i = (size_t)c * e_local + e;
-      const int n = r.chunk_counts[i];
-      r.chunk_counts[i] = at;
-      at += n;
-    }
-  }
+  publish_tiles((int)threadIdx.x < e_local ? sum_chunks(r, chunks, e_local) : 0, e_local, plan, r, s_off, s_tp, s_cnt,
+                s_wave);
 }
-// ... and the places.
+// ... and the places, behind those of the chunks before.
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_place_kernel(const int32_t* __restrict__ ids, int picks, int k, int e_local, int offset, Routes r) {
+sort_place_kernel(const int32_t* __restrict__ ids, const float* __restrict__ weights, int picks, int chunk, int k,
+                  int e_local, int offset, Routes r) {
   __shared__ int s_pos[MAX_EXPERTS];
-  const int tid = threadIdx.x, p0 = blockIdx.x * SORT_CHUNK;
-  if (tid < e_local) s_pos[tid] = r.chunk_counts[(size_t)blockIdx.x * e_local + tid];
+  const int tid = threadIdx.x, p0 = blockIdx.x * chunk;
+  if (tid < e_local) s_pos[tid] = r.offsets[tid] + sum_chunks(r, blockIdx.x, e_local);
   __syncthreads();
-  place_picks(ids, p0, min(picks, p0 + SORT_CHUNK), k, e_local, offset, s_pos, r);
+  place_picks(ids, weights, p0, min(picks, p0 + chunk), k, e_local, offset, s_pos, r);
 }
 
 // GEMM1 and SwiGLU of (route tile, NP pairs of 16 gate and 16 up rows): rows
@@ -767,7 +779,7 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
     }
 #pragma unroll
     for (int f = 0; f < FR; ++f) {
-      const int t = (r.route_pick[tile.y + min(16 * f + (lane & 15), tile.z - 1)] & PICK_MASK) / a.k;
+      const int t = r.route_token[tile.y + min(16 * f + (lane & 15), tile.z - 1)] & TOKEN_MASK;
       st.x[f] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
       st.xs[f] = a.xs + t;
     }
@@ -788,12 +800,11 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
 
 // Four columns of a route's W2 c, times its weight: to Y, or to the output row of a
 // token that has no other local pick.
-__device__ __forceinline__ void store_y(const ExpertsW4& a, const Routes& r, float* __restrict__ Y, int route, int col,
-                                        const v4f& v) {
-  const int rp = r.route_pick[route], pick = rp & PICK_MASK;
-  const v4f y = v * a.weights[pick];
-  if (rp < 0)  // 0 + y, as the combine's sum of one: -0 becomes +0
-    *reinterpret_cast<uint2*>(a.out + (size_t)(pick / a.k) * a.H + col) =
+__device__ __forceinline__ void store_y(const ExpertsW4& a, float* __restrict__ Y, int route, int token, float weight,
+                                        int col, const v4f& v) {
+  const v4f y = v * weight;
+  if (token < 0)  // 0 + y, as the combine's sum of one: -0 becomes +0
+    *reinterpret_cast<uint2*>(a.out + (size_t)(token & TOKEN_MASK) * a.H + col) =
         make_uint2(bf16_pair(y[0] + 0.0f, y[1] + 0.0f), bf16_pair(y[2] + 0.0f, y[3] + 0.0f));
   else
     *reinterpret_cast<float4*>(Y + (size_t)route * a.H + col) = make_float4(y[0], y[1], y[2], y[3]);
@@ -828,7 +839,8 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
     st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
       const int m = 16 * f + (lane & 15);
       if (m >= tile.z) return;
-      store_y(a, r, Y, tile.y + m, (j * NT + p) * 16 + 4 * (lane >> 4), y[0]);
+      store_y(a, Y, tile.y + m, r.route_token[tile.y + m], r.route_weight[tile.y + m], (j * NT + p) * 16 + 4 * (lane >> 4),
+              y[0]);
     });
   }
 }
@@ -866,7 +878,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
     constexpr int NC = decltype(ncc)::value;
     v4f acc[4][NC];
     tile_product<NC>(s, w, a.H, a.x, a.xs, 1, a.T, [&](int m) {
-      return (r.route_pick[tile.y + min(m, tile.z - 1)] & PICK_MASK) / a.k;
+      return r.route_token[tile.y + min(m, tile.z - 1)] & TOKEN_MASK;
     }, acc);
     // c in place of the gate's results, and the waves' largest magnitudes per route.
 #pragma unroll
@@ -924,6 +936,10 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
 #pragma unroll
   for (int n = 0; n < 4; ++n)
     w[n] = a.w2 + ((size_t)tile.x * tiles + min(nb * 16 + rw * 4 + n, tiles - 1)) * KC * W4_CHUNK_BYTES;
+  if (tid < TILE_MAX_M) {  // for the epilogue, behind the product's barriers
+    s.token[tid] = r.route_token[tile.y + min(tid, tile.z - 1)];
+    s.weight[tid] = r.route_weight[tile.y + min(tid, tile.z - 1)];
+  }
   by_rows(tile.z, [&](auto ncc) __attribute__((always_inline)) {
     constexpr int NC = decltype(ncc)::value;
     v4f acc[4][NC];
@@ -932,10 +948,12 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
     for (int c = 0; c < NC; ++c) {
       const int m = (cw * NC + c) * 16 + (lane & 15);
       if (m >= tile.z) continue;
+      const int token = s.token[m];
+      const float weight = s.weight[m];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int row = nb * 16 + rw * 4 + n;
-        if (row < tiles) store_y(a, r, Y, tile.y + m, row * 16 + 4 * (lane >> 4), acc[n][c]);
+        if (row < tiles) store_y(a, Y, tile.y + m, token, weight, row * 16 + 4 * (lane >> 4), acc[n][c]);
       }
     }
   });
@@ -962,7 +980,7 @@ experts_combine_kernel(const float* __restrict__ Y, const int32_t* __restrict__ 
 }
 
 struct ExpertsLayout {
-  size_t offsets, n_tiles, tiles, route_pick, pick_route, chunk_counts, cf, cq, cs, y, total;
+  size_t offsets, n_tiles, tiles, route_token, route_weight, pick_route, chunk_counts, cf, cq, cs, y, total;
 };
 // The smallest route tile sets the length of the tile list.
 constexpr int MIN_BM = 16;
@@ -970,7 +988,7 @@ size_t max_tiles(size_t picks, int e_local, int bm) {
   return (picks < (size_t)e_local ? picks : (size_t)e_local) + picks / bm;
 }
 ExpertsLayout experts_layout(int T, int H, int I, int e_local, int k) {
-  const size_t picks = (size_t)T * k, chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
+  const size_t picks = (size_t)T * k, chunks = SORT_MAX_CHUNKS;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -981,7 +999,8 @@ ExpertsLayout experts_layout(int T, int H, int I, int e_local, int k) {
   l.offsets = take(((size_t)e_local + 1) * 4);
   l.n_tiles = take(4);
   l.tiles = take(max_tiles(picks, e_local, MIN_BM) * 16);
-  l.route_pick = take(picks * 4);
+  l.route_token = take(picks * 4);
+  l.route_weight = take(picks * 4);
   l.pick_route = take(picks * 4);
   l.chunk_counts = take(chunks * e_local * 4);
   l.cf = take(picks * I * 4);
@@ -1046,7 +1065,7 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
         kernel<<<grid, TILE_THREADS, 0, stream>>>(x, xs, packed, T, N, K, base, out);
       });
     };
-    switch (linear_tile_nc(T, tiles, device_cus())) {
+    switch (linear_tile_nc(T, tiles, device_cus() * (2 / TILE_CW))) {
       case 1: tile(linear_w4_tile_kernel<1>, 1); break;
       case 2: tile(linear_w4_tile_kernel<2>, 2); break;
       case 3: tile(linear_w4_tile_kernel<3>, 3); break;
@@ -1070,9 +1089,10 @@ size_t experts_w4_workspace(int T, int H, int I, int e_local, int k) {
 
 hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream) {
   const ExpertsLayout l = experts_layout(a.T, a.H, a.I, a.e_local, a.k);
-  const Routes r = {reinterpret_cast<int32_t*>(ws + l.offsets),    reinterpret_cast<int32_t*>(ws + l.n_tiles),
-                    reinterpret_cast<int4*>(ws + l.tiles),         reinterpret_cast<int32_t*>(ws + l.route_pick),
-                    reinterpret_cast<int32_t*>(ws + l.pick_route), reinterpret_cast<int32_t*>(ws + l.chunk_counts)};
+  auto i32 = [&](size_t at) { return reinterpret_cast<int32_t*>(ws + at); };
+  const Routes r = {i32(l.offsets),     i32(l.n_tiles), reinterpret_cast<int4*>(ws + l.tiles),
+                    i32(l.route_token), reinterpret_cast<float*>(ws + l.route_weight), i32(l.pick_route),
+                    i32(l.chunk_counts)};
   float* Cf = reinterpret_cast<float*>(ws + l.cf);
   uint8_t* Cq = ws + l.cq;
   float* Cs = reinterpret_cast<float*>(ws + l.cs);
@@ -1080,17 +1100,17 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   const int picks = a.T * a.k;
   const bool tile = a.T > 256;
   const int fr = a.T <= 16 ? 1 : 2;
-  const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus()};
+  const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus() * (2 / TILE_CW)};
   hipError_t err;
-  if (picks <= SORT_CHUNK) {
-    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, plan, r);
+  if (picks <= SORT_SMALL) {
+    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
   } else {
-    const int chunks = (picks + SORT_CHUNK - 1) / SORT_CHUNK;
-    sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.e_local, a.offset, r);
+    const int chunk = sort_chunk(picks), chunks = (picks + chunk - 1) / chunk;
+    sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, chunk, a.e_local, a.offset, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
     sort_scan_kernel<<<1, SORT_THREADS, 0, stream>>>(chunks, a.e_local, plan, r);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, a.k, a.e_local, a.offset, r);
+    sort_place_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, chunk, a.k, a.e_local, a.offset, r);
   }
   if ((err = hipGetLastError()) != hipSuccess) return err;
   const size_t bound = max_tiles(picks, a.e_local, tile ? 2 * TILE_COLS : 16 * fr);

@@ -390,7 +390,7 @@ def test_experts_w4_layer_size(ops, cuda, T):
 
 @pytest.mark.gpu
 def test_experts_w4_many_experts_and_picks(ops, cuda):
-    """More picks than one workgroup sorts (8192), 1024 experts, up to 64 picks a token."""
+    """More picks than one workgroup sorts (2048), 1024 experts, up to 64 picks a token."""
     rng = np.random.default_rng(5)
     for T, E, k in ((130, 1024, 64), (2100, 40, 5), (8193, 3, 1)):
         case = _experts_case(rng, T, 128, 128, E, k, lambda r, t, kk, e: np.argsort(r.random((t, e)), axis=1)[:, :kk])
