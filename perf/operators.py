@@ -13,6 +13,7 @@ call, `run` is one call: of the framework's operator where `own` is set, of its 
 4-bit weights are OCP MXFP4: two e2m1 codes a byte (the lower index in the low half), an e8m0 scale for each 32.
 """
 
+import functools
 import importlib
 import math
 
@@ -26,7 +27,8 @@ H, I, E_GLOBAL, E_LOCAL = 7168, 2048, 256, 32
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
 
 
-def _ops():
+@functools.lru_cache(None)
+def _ops():  # a program imports it once
     return importlib.import_module("15642_moe_amd.ops")
 
 
