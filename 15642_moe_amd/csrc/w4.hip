@@ -237,23 +237,49 @@ struct Stream {
 #pragma unroll
         for (int b = 0; b < 4; ++b) ca[n][b] = a[n][b];
       }
-      if (c + 1 < c1) load(c + 1);
-      static_for<4>([&](auto bc) __attribute__((always_inline)) {
-        constexpr int b = decltype(bc)::value;
-        const int kb = c * W4_CHUNK_BLOCKS + b;
-        if (kb < KB) {
+      if constexpr (FR == 1) {
+        // This chunk's activations, then the next one's weights: loads return in order,
+        // and the wait for the former leaves the latter in flight.
+        u32x4 lo[4], hi[4];
+        float s[4];
 #pragma unroll
-          for (int f = 0; f < FR; ++f) {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK);
-            const u32x4 hi = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK + 64);
-            const float s = xs[f][(size_t)kb * xs_stride];
-            const v8i xb = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int b = 0; b < 4; ++b) fragment(min(c * W4_CHUNK_BLOCKS + b, KB - 1), 0, lo[b], hi[b], s[b]);
+        if (c + 1 < c1) load(c + 1);
+        static_for<4>([&](auto bc) __attribute__((always_inline)) {
+          constexpr int b = decltype(bc)::value;
+          if (c * W4_CHUNK_BLOCKS + b < KB) multiply<b>(0, ca, csc, lo[b], hi[b], s[b]);
+        });
+      } else {
+        // By K-blocks: the registers of a chunk's fragments would cost half of the waves.
+        if (c + 1 < c1) load(c + 1);
+        static_for<4>([&](auto bc) __attribute__((always_inline)) {
+          constexpr int b = decltype(bc)::value;
+          const int kb = c * W4_CHUNK_BLOCKS + b;
+          if (kb < KB) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][f] += mfma_w4<b>(ca[n][b], xb, csc[n], zero4) * s;
+            for (int f = 0; f < FR; ++f) {
+              u32x4 lo, hi;
+              float s;
+              fragment(kb, f, lo, hi, s);
+              multiply<b>(f, ca, csc, lo, hi, s);
+            }
           }
-        }
-      });
+        });
+      }
     }
+  }
+  __device__ __forceinline__ void fragment(int kb, int f, u32x4& lo, u32x4& hi, float& s) const {
+    lo = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK);
+    hi = *reinterpret_cast<const u32x4*>(x[f] + (size_t)kb * BLK + 64);
+    s = xs[f][(size_t)kb * xs_stride];
+  }
+  template <int B>
+  __device__ __forceinline__ void multiply(int f, const u32x4 (&ca)[NT][4], const int (&csc)[NT], const u32x4& lo,
+                                           const u32x4& hi, float s) {
+    const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
+    const v8i xb = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][f] += mfma_w4<B>(ca[n][B], xb, csc[n], zero4) * s;
   }
   // The workgroup's sums, entry (n, f) in the registers of the wave that owns
   // it: `own(entry)` is called for the entries of this wave, after the waves'
@@ -756,10 +782,24 @@ sort_place_kernel(const int32_t* __restrict__ ids, const float* __restrict__ wei
   place_picks(ids, weights, p0, min(picks, p0 + chunk), k, e_local, offset, s_pos, r);
 }
 
+__device__ __forceinline__ float4 swiglu(const v4f& gate, const v4f& up) {
+  auto one = [&](int i) { return up[i] / (1.0f + __expf(-up[i])) * gate[i]; };
+  return make_float4(one(0), one(1), one(2), one(3));
+}
+
+// f(the fragments of 16 that hold `rows`, MAX at most).
+template <int MAX, int N = 1, class F>
+__device__ __forceinline__ void by_frags(int rows, F&& f) {
+  if constexpr (N < MAX) {
+    if (rows > 16 * N) return by_frags<MAX, N + 1>(rows, f);
+  }
+  f(std::integral_constant<int, N>{});
+}
+
 // GEMM1 and SwiGLU of (route tile, NP pairs of 16 gate and 16 up rows): rows
 // [0, I) of W13 multiply, SiLU takes rows [I, 2 I).  Workgroups past the last
 // tile end at once.
-template <int NP, int FR>
+template <int NP, int MAXFR>
 __global__ void __launch_bounds__(512)
 experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
   extern __shared__ v4f s_part[];
@@ -771,29 +811,28 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
   for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
     if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
     const int4 tile = r.tiles[i];
-    Stream<2 * NP, FR> st;
+    by_frags<MAXFR>(tile.z, [&](auto frc) __attribute__((always_inline)) {
+      constexpr int FR = decltype(frc)::value;
+      Stream<2 * NP, FR> st;
 #pragma unroll
-    for (int n = 0; n < 2 * NP; ++n) {
-      const int row = j * NP + (n < NP ? n : a.I / 16 + n - NP);
-      st.w[n] = a.w13 + ((size_t)tile.x * tiles + row) * KC * W4_CHUNK_BYTES + lane * 16;
-    }
+      for (int n = 0; n < 2 * NP; ++n) {
+        const int row = j * NP + (n < NP ? n : a.I / 16 + n - NP);
+        st.w[n] = a.w13 + ((size_t)tile.x * tiles + row) * KC * W4_CHUNK_BYTES + lane * 16;
+      }
 #pragma unroll
-    for (int f = 0; f < FR; ++f) {
-      const int t = r.route_token[tile.y + min(16 * f + (lane & 15), tile.z - 1)] & TOKEN_MASK;
-      st.x[f] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
-      st.xs[f] = a.xs + t;
-    }
-    st.xs_stride = a.T;
-    st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
-    st.template reduce<2>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
-      const int m = 16 * f + (lane & 15);
-      if (m >= tile.z) return;
-      float4 c;
-      c.x = y[1][0] / (1.0f + __expf(-y[1][0])) * y[0][0];
-      c.y = y[1][1] / (1.0f + __expf(-y[1][1])) * y[0][1];
-      c.z = y[1][2] / (1.0f + __expf(-y[1][2])) * y[0][2];
-      c.w = y[1][3] / (1.0f + __expf(-y[1][3])) * y[0][3];
-      *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + (j * NP + p) * 16 + 4 * (lane >> 4)) = c;
+      for (int f = 0; f < FR; ++f) {
+        const int t = r.route_token[tile.y + min(16 * f + (lane & 15), tile.z - 1)] & TOKEN_MASK;
+        st.x[f] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
+        st.xs[f] = a.xs + t;
+      }
+      st.xs_stride = a.T;
+      st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
+      st.template reduce<2>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+        const int m = 16 * f + (lane & 15);
+        if (m >= tile.z) return;
+        *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + (j * NP + p) * 16 + 4 * (lane >> 4)) =
+            swiglu(y[0], y[1]);
+      });
     });
   }
 }
@@ -811,7 +850,7 @@ __device__ __forceinline__ void store_y(const ExpertsW4& a, float* __restrict__ 
 }
 
 // GEMM2 of (route tile, NT 16-row tiles of W2), times the pick's weight.
-template <int NT, int FR>
+template <int NT, int MAXFR>
 __global__ void __launch_bounds__(512)
 experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
                                      const float* __restrict__ Cs, float* __restrict__ Y) {
@@ -824,24 +863,185 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
   for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
     if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
     const int4 tile = r.tiles[i];
-    Stream<NT, FR> st;
+    by_frags<MAXFR>(tile.z, [&](auto frc) __attribute__((always_inline)) {
+      constexpr int FR = decltype(frc)::value;
+      Stream<NT, FR> st;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      st.w[n] = a.w2 + ((size_t)tile.x * tiles + j * NT + n) * KC * W4_CHUNK_BYTES + lane * 16;
+      for (int n = 0; n < NT; ++n)
+        st.w[n] = a.w2 + ((size_t)tile.x * tiles + j * NT + n) * KC * W4_CHUNK_BYTES + lane * 16;
 #pragma unroll
-    for (int f = 0; f < FR; ++f) {
-      const size_t row = tile.y + min(16 * f + (lane & 15), tile.z - 1);
-      st.x[f] = Cq + row * a.I + 16 * (lane >> 4);
-      st.xs[f] = Cs + row * KB;
-    }
-    st.xs_stride = 1;
-    st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
-    st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
-      const int m = 16 * f + (lane & 15);
-      if (m >= tile.z) return;
-      store_y(a, Y, tile.y + m, r.route_token[tile.y + m], r.route_weight[tile.y + m], (j * NT + p) * 16 + 4 * (lane >> 4),
-              y[0]);
+      for (int f = 0; f < FR; ++f) {
+        const size_t row = tile.y + min(16 * f + (lane & 15), tile.z - 1);
+        st.x[f] = Cq + row * a.I + 16 * (lane >> 4);
+        st.xs[f] = Cs + row * KB;
+      }
+      st.xs_stride = 1;
+      st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
+      st.template reduce<1>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+        const int m = 16 * f + (lane & 15);
+        if (m >= tile.z) return;
+        store_y(a, Y, tile.y + m, r.route_token[tile.y + m], r.route_weight[tile.y + m], (j * NT + p) * 16 + 4 * (lane >> 4),
+                y[0]);
+      });
     });
+  }
+}
+
+// ---------------------------------------------------------------------------
+// At most 64 picks in all: every workgroup sorts them itself, one per lane, and GEMM2
+// requantises and combines, so a call is two launches (T = 1: 26 us with the five of
+// the general path, whose kernels take 3 us each for nothing but their launch).
+// Rows of Cf are picks here.
+// ---------------------------------------------------------------------------
+constexpr int FEW_PICKS = 64;
+struct FewLds {
+  int pick[FEW_PICKS], expert[FEW_PICKS];  // the local picks, by expert, then pick
+};
+struct FewTile {
+  int expert, first, rows;  // rows places of FewLds::pick from `first` on
+};
+// Sorts the picks; returns a mask whose bits are the tiles' first places (tiles of at
+// most 16 routes of one expert), and the number of local picks in n.  Every wave calls it.
+__device__ __forceinline__ uint64_t few_sort(const ExpertsW4& a, FewLds& s, int& n) {
+  const int lane = threadIdx.x & 63, picks = a.T * a.k;
+  const int e = lane < picks ? local_expert(a.ids[lane], a.e_local, a.offset) : -1;
+  const uint64_t local = __ballot(e >= 0);
+  n = __popcll(local);
+  int rank = 0;
+  for (uint64_t m = local; m; m &= m - 1) {
+    const int q = __builtin_ctzll(m), o = __builtin_amdgcn_readlane(e, q);
+    rank += o < e || (o == e && q < lane) ? 1 : 0;
+  }
+  if (e >= 0) {  // all waves write the same
+    s.pick[rank] = lane;
+    s.expert[rank] = e;
+  }
+  __syncthreads();
+  const int mine = lane < n ? s.expert[lane] : -1, before = lane > 0 && lane < n ? s.expert[lane - 1] : -2;
+  const uint64_t starts = __ballot(lane < n && mine != before);
+  // the place within the expert's run: from the last start at or below this lane
+  const uint64_t below = starts & (~0ull >> (63 - lane));
+  const int from = below ? 63 - __builtin_clzll(below) : 0;
+  return __ballot(lane < n && ((lane - from) & 15) == 0);
+}
+__device__ __forceinline__ FewTile few_tile(const FewLds& s, uint64_t tiles, int i, int n) {
+  for (int j = 0; j < i; ++j) tiles &= tiles - 1;
+  const int first = __builtin_ctzll(tiles);
+  tiles &= tiles - 1;
+  return {s.expert[first], first, (tiles ? __builtin_ctzll(tiles) : n) - first};
+}
+
+// GEMM1 and SwiGLU of (tile, 16 gate and 16 up rows).
+__global__ void __launch_bounds__(512)
+few_gemm1_kernel(ExpertsW4 a, float* __restrict__ Cf) {
+  extern __shared__ v4f s_part[];
+  __shared__ FewLds s;
+  const int slices = a.I / 16, i = blockIdx.x / slices, j = blockIdx.x % slices;
+  int n;
+  const uint64_t tiles = few_sort(a, s, n);
+  if (i >= __popcll(tiles)) return;
+  const FewTile tile = few_tile(s, tiles, i, n);
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int KC = w4_chunks(a.H), expert = __builtin_amdgcn_readfirstlane(tile.expert);
+  Stream<2, 1> st;
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    st.w[g] = a.w13 + ((size_t)expert * (2 * slices) + g * slices + j) * KC * W4_CHUNK_BYTES + lane * 16;
+  const int t = s.pick[tile.first + min(lane & 15, tile.rows - 1)] / a.k;
+  st.x[0] = a.x + (size_t)t * a.H + 16 * (lane >> 4);
+  st.xs[0] = a.xs + t;
+  st.xs_stride = a.T;
+  st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), a.H / BLK);
+  st.reduce<2>(s_part, wave, waves, [&](int, int, const v4f* y) {
+    if ((lane & 15) >= tile.rows) return;
+    *reinterpret_cast<float4*>(Cf + (size_t)s.pick[tile.first + (lane & 15)] * a.I + j * 16 + 4 * (lane >> 4)) =
+        swiglu(y[0], y[1]);
+  });
+}
+
+// GEMM2 of 32 output columns of every token: per tile the workgroup requantises its
+// rows of Cf into LDS (each of the H / 32 workgroups does: 2048 elements a route), wave
+// (nt, cw) multiplies weight tile nt with chunks cw, cw + 4, ..., the parts are added in K
+// order, and the picks' results, times their weights, are kept until all are there.
+constexpr int FEW_THREADS = 512, FEW_MAX_I = 2048;
+__global__ void __launch_bounds__(FEW_THREADS)
+few_gemm2_kernel(ExpertsW4 a, const float* __restrict__ Cf) {
+  extern __shared__ __align__(16) uint8_t s_x[];  // codes [16][I], 16-byte pieces at piece ^ (row & 7)
+  __shared__ FewLds s;
+  __shared__ float s_xs[16][FEW_MAX_I / BLK];
+  __shared__ v4f s_part[8][64];
+  __shared__ float s_y[FEW_PICKS][33];
+  int n;
+  uint64_t tiles = few_sort(a, s, n);
+  const int tid = threadIdx.x, lane = tid & 63, nt = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int cw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), i16 = lane & 15, g = lane >> 4;
+  const int KC = w4_chunks(a.I), KB = a.I / BLK, n_tiles = __popcll(tiles);
+  const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
+  u32x4 w[4];
+  int sc = 0;
+  auto load = [&](int expert, int c) {
+    const uint8_t* p = a.w2 + (((size_t)expert * (a.H / 16) + blockIdx.x * 2 + nt) * KC + c) * W4_CHUNK_BYTES;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      w[b] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + (uint32_t)(b * W4_BLOCK_BYTES + lane * 16)));
+    sc = __builtin_nontemporal_load(
+        reinterpret_cast<const int*>(p + (uint32_t)(W4_CHUNK_BLOCKS * W4_BLOCK_BYTES + lane * 4)));
+  };
+  for (int i = 0; i < n_tiles; ++i) {
+    const FewTile tile = few_tile(s, tiles, 0, n);
+    tiles &= tiles - 1;
+    const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
+    if (cw < KC) load(expert, cw);  // in flight over the requantisation
+    for (int u = tid >> 4; u < tile.rows * KB; u += FEW_THREADS / 16) {
+      const int m = u / KB, kb = u - m * KB, sub = tid & 15;
+      float f[8], scale;
+      load8<DT_F32>(Cf, (size_t)s.pick[tile.first + m] * a.I + kb * BLK + sub * 8, f);
+      const uint2 o = quant8(f, scale);
+      *reinterpret_cast<uint2*>(s_x + m * a.I + kb * BLK + (((sub >> 1) ^ (m & 7)) << 4) + (sub & 1) * 8) = o;
+      if (sub == 0) s_xs[m][kb] = scale;
+    }
+    __syncthreads();
+    v4f acc = zero4;
+    const int m = min(i16, tile.rows - 1);
+    for (int c = cw; c < KC; c += 4) {
+      if (c > cw) load(expert, c);
+      static_for<4>([&](auto bc) __attribute__((always_inline)) {
+        constexpr int b = decltype(bc)::value;
+        const int kb = c * W4_CHUNK_BLOCKS + b;
+        if (kb < KB) {
+          const uint8_t* xb = s_x + m * a.I + kb * BLK;
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(xb + ((g ^ (m & 7)) << 4));
+          const u32x4 hi = *reinterpret_cast<const u32x4*>(xb + (((g + 4) ^ (m & 7)) << 4));
+          const v8i x = __builtin_bit_cast(v8i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc += mfma_w4<b>(w[b], x, sc, zero4) * s_xs[m][kb];
+        }
+      });
+    }
+    s_part[nt * 4 + cw][lane] = acc;
+    __syncthreads();
+    if (tid < 128) {  // threads (nt, lane): the four columns of one route
+      const int h = tid >> 6;
+      v4f y = s_part[h * 4][lane];
+      for (int c = 1; c < 4; ++c) y += s_part[h * 4 + c][lane];
+      if (i16 < tile.rows) {
+        const int p = s.pick[tile.first + i16];
+        y *= a.weights[p];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s_y[p][h * 16 + 4 * g + v] = y[v];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < a.T * 16; i += FEW_THREADS) {
+    const int t = i >> 4, col = (i & 15) * 2;
+    float y0 = 0.0f, y1 = 0.0f;
+    for (int p = t * a.k; p < (t + 1) * a.k; ++p)
+      if (local_expert(a.ids[p], a.e_local, a.offset) >= 0) {
+        y0 += s_y[p][col];
+        y1 += s_y[p][col + 1];
+      }
+    *reinterpret_cast<uint32_t*>(a.out + (size_t)t * a.H + blockIdx.x * 32 + col) = bf16_pair(y0, y1);
   }
 }
 
@@ -1054,10 +1254,16 @@ static int linear_tile_nc(int T, int tiles, int cus) {
   return best;
 }
 
+// Waves that share KC chunks: up to 8, each with as many but for the last.
+static int stream_waves(int KC) {
+  const int per = (KC + 7) / 8;
+  return (KC + per - 1) / per;
+}
+
 hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* packed, int T, int N, int K,
                             uint16_t* out, hipStream_t stream) {
   const int tiles = w4_tiles(N), KC = w4_chunks(K);
-  const int waves = KC < 8 ? KC : 8;
+  const int waves = stream_waves(KC);
   if (T > 64) {
     auto tile = [&](auto kernel, int nc) {
       const size_t items = (size_t)((tiles + 15) / 16) * ((T + TILE_COLS * nc - 1) / (TILE_COLS * nc));
@@ -1098,10 +1304,18 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   float* Cs = reinterpret_cast<float*>(ws + l.cs);
   float* Y = reinterpret_cast<float*>(ws + l.y);
   const int picks = a.T * a.k;
+  hipError_t err;
+  if (picks <= FEW_PICKS && a.I <= FEW_MAX_I) {
+    const size_t tiles = max_tiles(picks, a.e_local, 16);
+    const int w = stream_waves(w4_chunks(a.H));
+    few_gemm1_kernel<<<(unsigned)(tiles * (a.I / 16)), 64 * w, w * 2 * 1024, stream>>>(a, Cf);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    few_gemm2_kernel<<<a.H / 32, FEW_THREADS, 16 * a.I, stream>>>(a, Cf);
+    return hipGetLastError();
+  }
   const bool tile = a.T > 256;
   const int fr = a.T <= 16 ? 1 : 2;
   const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus() * (2 / TILE_CW)};
-  hipError_t err;
   if (picks <= SORT_SMALL) {
     sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
   } else {
@@ -1131,7 +1345,7 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
     experts_combine_kernel<<<dim3(a.T, (a.H + 1023) / 1024), 256, 0, stream>>>(Y, r.pick_route, a.H, a.k, a.out);
     return hipGetLastError();
   }
-  auto waves_of = [](int K) { return w4_chunks(K) < 8 ? w4_chunks(K) : 8; };
+  auto waves_of = [](int K) { return stream_waves(w4_chunks(K)); };
   {
     const int w = waves_of(a.H);
     const unsigned grid = grid_of(a.I / 16);
