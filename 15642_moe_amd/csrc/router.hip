@@ -52,21 +52,54 @@ __device__ __forceinline__ uint32_t open_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// Reductions over the wave, uniform results: within rows of 16 lanes by DPP moves (lanes
+// l ^ 1, l ^ 2, l ^ 7, l ^ 15: no LDS round trip), over the rows by readlane.
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(dpp<CTRL>(__float_as_int(x)));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  return __hiloint2double(dpp<CTRL>(__double2hiint(x)), dpp<CTRL>(__double2loint(x)));
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int l) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+}
+__device__ __forceinline__ float lane_of(float x, int l) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), l),
+                          __builtin_amdgcn_readlane(__double2loint(x), l));
+}
+// The identity 0 as the old value lets each move and its maximum be one instruction.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
-  return x;
+  x = dpp_max<DPP_MIRROR>(dpp_max<DPP_HALF_MIRROR>(dpp_max<DPP_XOR2>(dpp_max<DPP_XOR1>(x))));
+  return max(max(lane_of(x, 0), lane_of(x, 16)), max(lane_of(x, 32), lane_of(x, 48)));
 }
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+  x = fmaxf(x, dpp<DPP_XOR1>(x));
+  x = fmaxf(x, dpp<DPP_XOR2>(x));
+  x = fmaxf(x, dpp<DPP_HALF_MIRROR>(x));
+  x = fmaxf(x, dpp<DPP_MIRROR>(x));
+  return fmaxf(fmaxf(lane_of(x, 0), lane_of(x, 16)), fmaxf(lane_of(x, 32), lane_of(x, 48)));
 }
 template <class F>
 __device__ __forceinline__ F wave_sum(F x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-  return x;
+  x += dpp<DPP_XOR1>(x);
+  x += dpp<DPP_XOR2>(x);
+  x += dpp<DPP_HALF_MIRROR>(x);
+  x += dpp<DPP_MIRROR>(x);
+  return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
 }
 
 // exp(x - m) of a softmax; the maximum's own is 1, also where it is +inf.
@@ -79,7 +112,7 @@ __device__ __forceinline__ F exp_below(float x, float m) {
 template <int EPL, int DT, bool SOFTMAX>
 __global__ void __launch_bounds__(64 * WAVES)
 route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const float* __restrict__ bias, int T, int E,
-                  int k, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                  int k, int n_group, int lanes_per_group, int topk_group, int group_top, int renormalize, float scale,
                   float* __restrict__ weights, int32_t* __restrict__ ids) {
   __shared__ float s_v[WAVES][64 * EPL];
   __shared__ float s_sel[WAVES][64];
@@ -126,30 +159,58 @@ route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const floa
 #pragma unroll
   for (int j = 0; j < EPL; ++j) key[j] = open_key(v[j]);
   if (n_group > 1) {
-    // Lane g scores group g; a closed second place adds nothing.
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) s_v[wave][lane * EPL + j] = v[j];
-    __syncthreads();
     const int gs = E / n_group;
     float m1 = -INFINITY, m2 = -INFINITY;
-    if (lane < n_group)
-      for (int i = 0; i < gs; ++i) {
-        const float y = s_v[wave][lane * gs + i];
-        m2 = fmaxf(m2, fminf(m1, y));
-        m1 = fmaxf(m1, y);
-      }
-    const float score = (group_top == 2 && m2 > -INFINITY) ? m1 + m2 : m1;
-    const uint32_t gkey = open_key(score);
-    int rank = 0;
-    for (int g = 0; g < n_group; ++g) {
-      const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)gkey, g);
-      rank += (o > gkey || (o == gkey && g < lane)) ? 1 : 0;
-    }
-    const uint64_t kept = __ballot(lane < n_group && rank < topk_group);
+    auto score = [&] {  // a closed second place adds nothing
+      return open_key((group_top == 2 && m2 > -INFINITY) ? m1 + m2 : m1);
+    };
+    auto add = [&](float y) {
+      m2 = fmaxf(m2, fminf(m1, y));
+      m1 = fmaxf(m1, y);
+    };
+    auto merge = [&](float o1, float o2) {
+      m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+      m1 = fmaxf(m1, o1);
+    };
+    if (lanes_per_group > 0) {
+      // A group is a power of two of whole lanes, at most a row's 16: its lanes merge
+      // their two largest by DPP moves.
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = lane * EPL + j;
-      if (e >= E || !((kept >> (e / gs)) & 1u)) key[j] = 0u;
+      for (int j = 0; j < EPL; ++j) add(v[j]);
+      if (lanes_per_group > 1) merge(dpp<DPP_XOR1>(m1), dpp<DPP_XOR1>(m2));
+      if (lanes_per_group > 2) merge(dpp<DPP_XOR2>(m1), dpp<DPP_XOR2>(m2));
+      if (lanes_per_group > 4) merge(dpp<DPP_HALF_MIRROR>(m1), dpp<DPP_HALF_MIRROR>(m2));
+      if (lanes_per_group > 8) merge(dpp<DPP_MIRROR>(m1), dpp<DPP_MIRROR>(m2));
+      const uint32_t gkey = score();
+      const int mine = lane / lanes_per_group;
+      int rank = 0;
+      for (int g = 0; g < n_group; ++g) {
+        const uint32_t o = lane_of(gkey, g * lanes_per_group);
+        rank += (o > gkey || (o == gkey && g < mine)) ? 1 : 0;
+      }
+      if (rank >= topk_group || mine >= n_group) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) key[j] = 0u;
+      }
+    } else {
+      // Lane g scores group g from LDS.
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) s_v[wave][lane * EPL + j] = v[j];
+      __syncthreads();
+      if (lane < n_group)
+        for (int i = 0; i < gs; ++i) add(s_v[wave][lane * gs + i]);
+      const uint32_t gkey = score();
+      int rank = 0;
+      for (int g = 0; g < n_group; ++g) {
+        const uint32_t o = lane_of(gkey, g);
+        rank += (o > gkey || (o == gkey && g < lane)) ? 1 : 0;
+      }
+      const uint64_t kept = __ballot(lane < n_group && rank < topk_group);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        const int e = lane * EPL + j;
+        if (e >= E || !((kept >> (e / gs)) & 1u)) key[j] = 0u;
+      }
     }
   }
 
@@ -299,9 +360,13 @@ hipError_t launch_route_topk(const void* logits, int dtype, size_t row_stride, c
                              int softmax, int n_group, int topk_group, int group_top, int renormalize, float scale,
                              float* weights, int32_t* ids, hipStream_t stream) {
   return dispatch(E, dtype, softmax, [&](auto epl, auto dt, auto sm) {
+    constexpr int EPL = decltype(epl)::value;
+    const int gs = E / n_group, lanes = gs / EPL;
+    const bool whole = gs % EPL == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0;
     route_topk_kernel<decltype(epl)::value, decltype(dt)::value, decltype(sm)::value>
-        <<<(T + WAVES - 1) / WAVES, 64 * WAVES, 0, stream>>>(logits, row_stride, bias, T, E, k, n_group, topk_group,
-                                                             group_top, renormalize, scale, weights, ids);
+        <<<(T + WAVES - 1) / WAVES, 64 * WAVES, 0, stream>>>(logits, row_stride, bias, T, E, k, n_group,
+                                                             whole ? lanes : 0, topk_group, group_top, renormalize,
+                                                             scale, weights, ids);
   });
 }
 
