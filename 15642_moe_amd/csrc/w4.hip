@@ -120,40 +120,58 @@ quantize_w4_kernel(const void* __restrict__ w, size_t groups, uint8_t* __restric
 // e4m3(clamp(x / scale, +-448)), the rule of the producer and of the experts'
 // own requantisation.  16 lanes a block, 8 columns each.
 // ---------------------------------------------------------------------------
+// x / s correctly rounded wherever its e4m3 code can tell: from y = RN(1 / s) two
+// steps of remainder and correction (Markstein's: the second starts from a quotient
+// within an ulp), five operations where the IEEE division takes about ten.  x's sign is
+// put back (the correction turns -0 into +0).  |x| is at most the block's maximum, so the
+// quotient is at most 448 and an ulp or two, which e4m3 rounds to 448: no clamp.
+// s is the scale clamped to FLT_MAX: beside an infinite scale (y = 0) finite elements
+// become 0; infinities and NaN become NaN.
+__device__ __forceinline__ float quot(float x, float s, float y) {
+  const float q0 = x * y;
+  const float q1 = __builtin_fmaf(__builtin_fmaf(-q0, s, x), y, q0);
+  return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-q1, s, x), y, q1), x);
+}
+__device__ __forceinline__ uint32_t quot4_e4m3(float a, float b, float c, float d, float s, float y) {
+  return cvt4_e4m3(quot(a, s, y), quot(b, s, y), quot(c, s, y), quot(d, s, y));
+}
+// Scale of a block with the largest magnitude m, and what quot takes of it.
+__device__ __forceinline__ float block_scale(float m, float& s, float& y) {
+  const float sc = fmaxf(m / E4M3_MAX, 1.0e-8f);
+  s = fminf(sc, __FLT_MAX__);
+  y = 1.0f / sc;
+  return sc;
+}
+
 __device__ __forceinline__ uint2 quant8(const float (&f)[8], float& sc) {
   float m = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-  sc = fmaxf(m / E4M3_MAX, 1.0e-8f);
-  auto q = [&](float x) {  // a NaN (an infinity in its block) stays one
-    const float v = x / sc;
-    return v > E4M3_MAX ? E4M3_MAX : v < -E4M3_MAX ? -E4M3_MAX : v;
-  };
-  uint2 o;
-  o.x = cvt4_e4m3(q(f[0]), q(f[1]), q(f[2]), q(f[3]));
-  o.y = cvt4_e4m3(q(f[4]), q(f[5]), q(f[6]), q(f[7]));
-  return o;
+  float s, y;
+  sc = block_scale(m, s, y);
+  return make_uint2(quot4_e4m3(f[0], f[1], f[2], f[3], s, y), quot4_e4m3(f[4], f[5], f[6], f[7], s, y));
 }
 
-template <int DT>
+// A workgroup takes 16 rows x G blocks: a row's G blocks are read at once, and a block's
+// 16 scales are one line of [K / 128, T].
+template <int DT, int G>
 __global__ void __launch_bounds__(256)
 quant_act_kernel(const void* __restrict__ x, size_t row_stride, int T, int KB, uint8_t* __restrict__ codes,
                  float* __restrict__ scale) {
-  const size_t n = (size_t)T * KB;  // (row, block)
-  const int sub = threadIdx.x & 15;
-  for (size_t u0 = (size_t)blockIdx.x * 16; u0 < n; u0 += (size_t)gridDim.x * 16) {
-    const size_t u = u0 + (threadIdx.x >> 4);
-    const bool active = u < n;
-    const size_t t = active ? u / KB : 0;
-    const int kb = active ? (int)(u % KB) : 0;
-    float f[8], sc;
-    load8<DT>(x, t * row_stride + (size_t)kb * BLK + sub * 8, f);
-    const uint2 o = quant8(f, sc);
-    if (active) {
-      *reinterpret_cast<uint2*>(codes + (t * KB + kb) * BLK + sub * 8) = o;
-      if (sub == 0) scale[(size_t)kb * T + t] = sc;
+  const int t = blockIdx.x * 16 + (threadIdx.x >> 4), sub = threadIdx.x & 15, kb0 = blockIdx.y * G;
+  const size_t row = (size_t)min(t, T - 1) * row_stride;
+  float f[G][8];
+#pragma unroll
+  for (int i = 0; i < G; ++i) load8<DT>(x, row + (size_t)min(kb0 + i, KB - 1) * BLK + sub * 8, f[i]);
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    float sc;
+    const uint2 o = quant8(f[i], sc);
+    if (t < T && kb0 + i < KB) {
+      *reinterpret_cast<uint2*>(codes + ((size_t)t * KB + kb0 + i) * BLK + sub * 8) = o;
+      if (sub == 0) scale[(size_t)(kb0 + i) * T + t] = sc;
     }
   }
 }
@@ -1101,15 +1119,12 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int m = (cw * NC + c) * 16 + (lane & 15);
-      const float sc = fmaxf(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])) / E4M3_MAX, 1.0e-8f);
-      auto q = [&](float x) {
-        const float v = x / sc;
-        return v > E4M3_MAX ? E4M3_MAX : v < -E4M3_MAX ? -E4M3_MAX : v;
-      };
+      float qs, qy;
+      const float sc = block_scale(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])), qs, qy);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
         *reinterpret_cast<uint32_t*>(codes + tile_slot(m, 2 * rw + p) + 4 * g) =
-            cvt4_e4m3(q(acc[p][c][0]), q(acc[p][c][1]), q(acc[p][c][2]), q(acc[p][c][3]));
+            quot4_e4m3(acc[p][c][0], acc[p][c][1], acc[p][c][2], acc[p][c][3], qs, qy);
       if (rw == 0 && g == 0 && m < tile.z) Cs[(size_t)(tile.y + m) * IB + nb] = sc;
     }
     __syncthreads();
@@ -1233,11 +1248,19 @@ hipError_t launch_quantize_w4(const void* w, int dtype, size_t groups, uint8_t* 
 
 hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, int K, uint8_t* codes, float* scale,
                             hipStream_t stream) {
-  const size_t blocks = ((size_t)T * (K / BLK) + 15) / 16;
-  const unsigned grid = (unsigned)(blocks < MAX_GRID ? blocks : MAX_GRID);
-  if (dtype == DT_F32) quant_act_kernel<DT_F32><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
-  else if (dtype == DT_BF16) quant_act_kernel<DT_BF16><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
-  else quant_act_kernel<DT_F16><<<grid, 256, 0, stream>>>(x, row_stride, T, K / BLK, codes, scale);
+  const int KB = K / BLK, rows = (T + 15) / 16;
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    // Four blocks a thread where that leaves two workgroups a CU (T = 8192, K = 7168:
+    // 48 us with one of whole rows' blocks in turn, 38 with four).
+    if ((size_t)rows * ((KB + 3) / 4) >= 2 * (size_t)device_cus())
+      quant_act_kernel<DT, 4><<<dim3(rows, (KB + 3) / 4), 256, 0, stream>>>(x, row_stride, T, KB, codes, scale);
+    else
+      quant_act_kernel<DT, 1><<<dim3(rows, KB), 256, 0, stream>>>(x, row_stride, T, KB, codes, scale);
+  };
+  if (dtype == DT_F32) launch(std::integral_constant<int, DT_F32>{});
+  else if (dtype == DT_BF16) launch(std::integral_constant<int, DT_BF16>{});
+  else launch(std::integral_constant<int, DT_F16>{});
   return hipGetLastError();
 }
 
