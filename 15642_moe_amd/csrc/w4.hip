@@ -548,6 +548,17 @@ __device__ __forceinline__ int xcd_item(int base, int n_work) {
   const int q = blockIdx.x / XCDS, i = (int)(blockIdx.x % XCDS) * per + q;
   return q < per && i < n ? base + i : -1;
 }
+// The i-th item of nblk weight blocks x nt activation tiles: bands of up to 8 tiles, in a
+// band block after block, so that the tiles that read one block's weights are neighbours,
+// and a band's activations stay in the L2 from one block to the next.  (Weights of
+// 131072 rows, T = 128, K = 7168: tile after tile 154 us, so 147; T = 1501, N = 7168,
+// K = 2048: 34.8 and 32.0.)
+__device__ __forceinline__ void banded(int i, int nblk, int nt, int& nb, int& tile) {
+  constexpr int BAND = 8;
+  const int band = i / (BAND * nblk), r = i - band * (BAND * nblk), width = min(BAND, nt - band * BAND);
+  nb = r / width;
+  tile = band * BAND + (r - nb * width);
+}
 // Launches for `items` items at most, each below 2^32 threads: f(grid, first item).
 template <class F>
 void by_grids(size_t items, F&& f) {
@@ -565,9 +576,12 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
   const int tid = threadIdx.x, lane = tid & 63;
   const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(K), tiles = w4_tiles(N), blocks = (tiles + 15) / 16;
-  const int item = xcd_item(base, blocks * ((T + TILE_COLS * NC - 1) / (TILE_COLS * NC)));
+  const int token_tiles = (T + TILE_COLS * NC - 1) / (TILE_COLS * NC);
+  const int item = xcd_item(base, blocks * token_tiles);
   if (item < 0) return;
-  const int nb = item % blocks, t0 = item / blocks * (TILE_COLS * NC);
+  int nb, tt;
+  banded(item, blocks, token_tiles, nb, tt);
+  const int t0 = tt * (TILE_COLS * NC);
   const uint8_t* w[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n)
@@ -623,7 +637,8 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
 struct Routes {
   int32_t* offsets;      // [e_local + 1] first route of each expert; the last: their number
   int32_t* n_tiles;      // [1]
-  int4* tiles;           // {expert, first route, routes, 0}
+  int4* tiles;           // {expert, first route, routes, first tile of the expert}
+  int32_t* tile_count;   // tiles of each tile's expert
   int32_t* route_token;  // [T k] token of each route; bit 31: its only local one
   float* route_weight;   // [T k]
   int32_t* pick_route;   // [T k], -1 for picks of other experts
@@ -680,15 +695,29 @@ __device__ __forceinline__ void publish_tiles(int cnt, int e_local, const TilePl
   int total, tiles, bm = plan.bm;
   const int off = block_scan(cnt, s_wave, total);
   if (bm == 0) {
+    // The sums of every size's tiles at once.
+    constexpr int SIZES = TILE_MAX_NC - 1;
+    __shared__ int s_sum[SIZES];
+    if (e < SIZES) s_sum[e] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SIZES; ++i) {
+      const int m = (i + 2) * TILE_COLS;
+      int n = (cnt + m - 1) / m;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+      if ((e & 63) == 0 && n > 0) atomicAdd(&s_sum[i], n);
+    }
+    __syncthreads();
     float least = 0.0f;
-    for (int m = TILE_MAX_M; m >= 2 * TILE_COLS; m -= TILE_COLS) {
-      block_scan((cnt + m - 1) / m, s_wave, tiles);
-      const float item = (float)total / (float)(TILE_COLS * max(tiles, 1)) + 1.2f;
-      const float cost = item * ((float)((tiles * plan.n1 + plan.cus - 1) / plan.cus * plan.k1) +
-                                 (float)((tiles * plan.n2 + plan.cus - 1) / plan.cus * plan.k2));
-      if (m == TILE_MAX_M || cost < least) {
+    for (int i = SIZES - 1; i >= 0; --i) {
+      const int n = max(s_sum[i], 1);
+      const float item = (float)total / (float)(TILE_COLS * n) + 1.2f;
+      const float cost = item * ((float)((n * plan.n1 + plan.cus - 1) / plan.cus * plan.k1) +
+                                 (float)((n * plan.n2 + plan.cus - 1) / plan.cus * plan.k2));
+      if (i == SIZES - 1 || cost < least) {
         least = cost;
-        bm = m;
+        bm = (i + 2) * TILE_COLS;
       }
     }
   }
@@ -713,7 +742,8 @@ __device__ __forceinline__ void publish_tiles(int cnt, int e_local, const TilePl
     }
     const int n = s_cnt[lo], nt = (n + bm - 1) / bm;
     const int per = (((n + 15) >> 4) + nt - 1) / nt * 16, m0 = (i - s_tp[lo]) * per;
-    r.tiles[i] = make_int4(lo, s_off[lo] + m0, min(per, n - m0), 0);
+    r.tiles[i] = make_int4(lo, s_off[lo] + m0, min(per, n - m0), s_tp[lo]);
+    r.tile_count[i] = nt;
   }
 }
 
@@ -1073,6 +1103,14 @@ __device__ __forceinline__ void by_rows(int rows, F&& f) {
   f(std::integral_constant<int, NC>{});
 }
 
+// The tile and weight block of an item: experts in turn, an expert's items banded.
+__device__ __forceinline__ int4 expert_item(const Routes& r, int item, int nblk, int& nb) {
+  const int i = item / nblk, first = r.tiles[i].w;
+  int tile;
+  banded(item - first * nblk, nblk, r.tile_count[i], nb, tile);
+  return r.tiles[first + tile];
+}
+
 // GEMM1, SwiGLU and the FP8 requantisation of (route tile, 128 columns of the
 // intermediate): wave rw's weight tiles are 32 gate and the same 32 up rows.
 __global__ void __launch_bounds__(TILE_THREADS, 2)
@@ -1081,8 +1119,8 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
   const int IB = a.I / BLK;
   const int item = xcd_item(base, *r.n_tiles * IB);
   if (item < 0) return;
-  const int nb = item % IB;
-  const int4 tile = r.tiles[item / IB];
+  int nb;
+  const int4 tile = expert_item(r, item, IB, nb);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(a.H), tiles = 2 * a.I / 16;
@@ -1142,8 +1180,8 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
   const int tiles = a.H / 16, blocks = (tiles + 15) / 16, KB = a.I / BLK;
   const int item = xcd_item(base, *r.n_tiles * blocks);
   if (item < 0) return;
-  const int nb = item % blocks;
-  const int4 tile = r.tiles[item / blocks];
+  int nb;
+  const int4 tile = expert_item(r, item, blocks, nb);
   const int tid = threadIdx.x, lane = tid & 63;
   const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int KC = w4_chunks(a.I);
@@ -1195,7 +1233,7 @@ experts_combine_kernel(const float* __restrict__ Y, const int32_t* __restrict__ 
 }
 
 struct ExpertsLayout {
-  size_t offsets, n_tiles, tiles, route_token, route_weight, pick_route, chunk_counts, cf, cq, cs, y, total;
+  size_t offsets, n_tiles, tiles, tile_count, route_token, route_weight, pick_route, chunk_counts, cf, cq, cs, y, total;
 };
 // The smallest route tile sets the length of the tile list.
 constexpr int MIN_BM = 16;
@@ -1214,6 +1252,7 @@ ExpertsLayout experts_layout(int T, int H, int I, int e_local, int k) {
   l.offsets = take(((size_t)e_local + 1) * 4);
   l.n_tiles = take(4);
   l.tiles = take(max_tiles(picks, e_local, MIN_BM) * 16);
+  l.tile_count = take(max_tiles(picks, e_local, MIN_BM) * 4);
   l.route_token = take(picks * 4);
   l.route_weight = take(picks * 4);
   l.pick_route = take(picks * 4);
@@ -1320,7 +1359,7 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   const ExpertsLayout l = experts_layout(a.T, a.H, a.I, a.e_local, a.k);
   auto i32 = [&](size_t at) { return reinterpret_cast<int32_t*>(ws + at); };
   const Routes r = {i32(l.offsets),     i32(l.n_tiles), reinterpret_cast<int4*>(ws + l.tiles),
-                    i32(l.route_token), reinterpret_cast<float*>(ws + l.route_weight), i32(l.pick_route),
+                    i32(l.tile_count),  i32(l.route_token), reinterpret_cast<float*>(ws + l.route_weight), i32(l.pick_route),
                     i32(l.chunk_counts)};
   float* Cf = reinterpret_cast<float*>(ws + l.cf);
   uint8_t* Cq = ws + l.cq;
