@@ -8,9 +8,8 @@
 //
 // An expert whose logit or v is -inf or NaN is closed: it is never picked (its
 // softmax score is 0).  Slots that no open expert fills hold id -1, weight 0.
-// The picks follow from comparisons of 32-bit values, so the 64-bit exponential
-// (about 50 f64 operations, which this GPU issues at the f32 rate) is what makes
-// them the same on every machine that rounds it once.
+// The picks follow from comparisons of 32-bit values, so the 64-bit exponential, rounded
+// once, is what makes them the same on every machine.
 //
 // Gradient of the weights, with p = s over the picks and P = sum p + 1e-20:
 //   ds_k = scale * (g_k - sum_j g_j p_j / P) / P   or   scale * g_k
@@ -42,6 +41,27 @@ __device__ __forceinline__ void store_f32_as(void* base, size_t i, float v) {
   if constexpr (DT == DT_F32) static_cast<float*>(base)[i] = v;
   else if constexpr (DT == DT_BF16) static_cast<uint16_t*>(base)[i] = v == v ? bf16_rne(v) : (uint16_t)0x7FC0;
   else static_cast<_Float16*>(base)[i] = (_Float16)v;
+}
+
+// P consecutive elements, in loads of up to 16 bytes (the pointer aligned to them).
+template <int DT, int P>
+__device__ __forceinline__ void load_all(const void* base, size_t i, float (&x)[P]) {
+  if constexpr (DT == DT_F32) {
+#pragma unroll
+    for (int j = 0; j < P; j += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i + j);
+      x[j] = f.x; x[j + 1] = f.y; x[j + 2] = f.z; x[j + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; j += 4) {
+      const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i + j);
+      const uint32_t h[4] = {u.x & 0xFFFFu, u.x >> 16, u.y & 0xFFFFu, u.y >> 16};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        x[j + q] = DT == DT_BF16 ? __uint_as_float(h[q] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h[q]);
+    }
+  }
 }
 
 // Order-preserving map to uint32; 0 (below every open expert's) for -inf and NaN.
@@ -102,30 +122,68 @@ __device__ __forceinline__ F wave_sum(F x) {
   return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
 }
 
-// exp(x - m) of a softmax; the maximum's own is 1, also where it is +inf.
-template <class F>
-__device__ __forceinline__ F exp_below(float x, float m) {
-  return x == m ? (F)1 : (F)exp((F)x - (F)m);
+// exp(x) to about 2^-52: x = n ln 2 + r with |r| <= ln(2) / 2 (ln 2 in two parts), and the
+// series of exp(r) to r^13 / 13! (what is left is under 2^-57).
+__device__ __forceinline__ double exp64(double x) {
+  x = fmin(fmax(x, -1100.0), 1100.0);  // past both ends of the range
+  const double n = rint(x * 0x1.71547652b82fep+0);
+  double r = fma(n, -0x1.62e42fefa3800p-1, x);
+  r = fma(n, -0x1.ef35793c76730p-45, r);
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
-// One wave per token; lane l holds experts EPL*l .. +EPL.
+// exp(x - m) of a softmax; the maximum's own is 1, also where it is +inf.
+__device__ __forceinline__ double exp64_below(float x, float m) { return x == m ? 1.0 : exp64((double)x - (double)m); }
+__device__ __forceinline__ float exp32_below(float x, float m) { return x == m ? 1.0f : expf(x - m); }
+
+// 1 / (1 + e), e = exp(-x) rounded once to 32 bits.
+__device__ __forceinline__ float sigmoid(float x) { return __fdiv_rn(1.0f, 1.0f + (float)exp64(-(double)x)); }
+
+struct RouteArgs {
+  const void* logits;
+  size_t row_stride;
+  const float* bias;
+  int T, E, k, n_group, lanes_per_group, topk_group, group_top, renormalize, vec;
+  float scale;
+  float* weights;
+  int32_t* ids;
+};
+template <int EPL>
+struct RouteLds {  // one wave's
+  float v[64 * EPL];
+  float sel[64];
+  int id[64];
+};
+// Orders a wave's own LDS writes and reads (which the hardware keeps in order).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Token t by one wave; lane l holds experts EPL*l .. +EPL.
 template <int EPL, int DT, bool SOFTMAX>
-__global__ void __launch_bounds__(64 * WAVES)
-route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const float* __restrict__ bias, int T, int E,
-                  int k, int n_group, int lanes_per_group, int topk_group, int group_top, int renormalize, float scale,
-                  float* __restrict__ weights, int32_t* __restrict__ ids) {
-  __shared__ float s_v[WAVES][64 * EPL];
-  __shared__ float s_sel[WAVES][64];
-  __shared__ int s_id[WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x * WAVES + wave;
-  const bool active = t < T;  // idle waves still reach the barriers
-  const size_t row = (size_t)(active ? t : T - 1) * row_stride;
-  float x[EPL], s[EPL], v[EPL];
+__device__ __forceinline__ void route_token(const RouteArgs& a, int t, RouteLds<EPL>& s) {
+  const int lane = threadIdx.x & 63;
+  const size_t row = (size_t)t * a.row_stride;
+  float x[EPL], sc[EPL], v[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane * EPL + j;
-    x[j] = e < E ? load_as_f32<DT>(logits, row + e) : -INFINITY;
+    x[j] = e < a.E ? load_as_f32<DT>(a.logits, row + e) : -INFINITY;
   }
   if constexpr (SOFTMAX) {
     float m = -INFINITY;
@@ -135,34 +193,32 @@ route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const floa
     double ex[EPL], sum = 0.0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      ex[j] = x[j] > -INFINITY ? exp_below<double>(x[j], m) : 0.0;
+      ex[j] = x[j] > -INFINITY ? exp64_below(x[j], m) : 0.0;
       sum += ex[j];
     }
     sum = wave_sum(sum);
+    const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] = sum > 0.0 ? (float)(ex[j] / sum) : 0.0f;
+    for (int j = 0; j < EPL; ++j) sc[j] = (float)(ex[j] * inv);
   } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const float e = (float)exp(-(double)x[j]);
-      s[j] = __fdiv_rn(1.0f, 1.0f + e);
-    }
+    for (int j = 0; j < EPL; ++j) sc[j] = sigmoid(x[j]);
   }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane * EPL + j;
-    v[j] = x[j] > -INFINITY ? (bias ? s[j] + bias[e] : s[j]) : -INFINITY;
+    v[j] = x[j] > -INFINITY ? (a.bias ? sc[j] + a.bias[e] : sc[j]) : -INFINITY;
     if (!(v[j] > -INFINITY)) v[j] = -INFINITY;
   }
 
   uint32_t key[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) key[j] = open_key(v[j]);
-  if (n_group > 1) {
-    const int gs = E / n_group;
+  if (a.n_group > 1) {
+    const int gs = a.E / a.n_group;
     float m1 = -INFINITY, m2 = -INFINITY;
     auto score = [&] {  // a closed second place adds nothing
-      return open_key((group_top == 2 && m2 > -INFINITY) ? m1 + m2 : m1);
+      return open_key((a.group_top == 2 && m2 > -INFINITY) ? m1 + m2 : m1);
     };
     auto add = [&](float y) {
       m2 = fmaxf(m2, fminf(m1, y));
@@ -172,44 +228,44 @@ route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const floa
       m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
       m1 = fmaxf(m1, o1);
     };
-    if (lanes_per_group > 0) {
+    if (a.lanes_per_group > 0) {
       // A group is a power of two of whole lanes, at most a row's 16: its lanes merge
       // their two largest by DPP moves.
 #pragma unroll
       for (int j = 0; j < EPL; ++j) add(v[j]);
-      if (lanes_per_group > 1) merge(dpp<DPP_XOR1>(m1), dpp<DPP_XOR1>(m2));
-      if (lanes_per_group > 2) merge(dpp<DPP_XOR2>(m1), dpp<DPP_XOR2>(m2));
-      if (lanes_per_group > 4) merge(dpp<DPP_HALF_MIRROR>(m1), dpp<DPP_HALF_MIRROR>(m2));
-      if (lanes_per_group > 8) merge(dpp<DPP_MIRROR>(m1), dpp<DPP_MIRROR>(m2));
+      if (a.lanes_per_group > 1) merge(dpp<DPP_XOR1>(m1), dpp<DPP_XOR1>(m2));
+      if (a.lanes_per_group > 2) merge(dpp<DPP_XOR2>(m1), dpp<DPP_XOR2>(m2));
+      if (a.lanes_per_group > 4) merge(dpp<DPP_HALF_MIRROR>(m1), dpp<DPP_HALF_MIRROR>(m2));
+      if (a.lanes_per_group > 8) merge(dpp<DPP_MIRROR>(m1), dpp<DPP_MIRROR>(m2));
       const uint32_t gkey = score();
-      const int mine = lane / lanes_per_group;
+      const int mine = lane / a.lanes_per_group;
       int rank = 0;
-      for (int g = 0; g < n_group; ++g) {
-        const uint32_t o = lane_of(gkey, g * lanes_per_group);
+      for (int g = 0; g < a.n_group; ++g) {
+        const uint32_t o = lane_of(gkey, g * a.lanes_per_group);
         rank += (o > gkey || (o == gkey && g < mine)) ? 1 : 0;
       }
-      if (rank >= topk_group || mine >= n_group) {
+      if (rank >= a.topk_group || mine >= a.n_group) {
 #pragma unroll
         for (int j = 0; j < EPL; ++j) key[j] = 0u;
       }
     } else {
       // Lane g scores group g from LDS.
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) s_v[wave][lane * EPL + j] = v[j];
-      __syncthreads();
-      if (lane < n_group)
-        for (int i = 0; i < gs; ++i) add(s_v[wave][lane * gs + i]);
+      for (int j = 0; j < EPL; ++j) s.v[lane * EPL + j] = v[j];
+      wave_fence();
+      if (lane < a.n_group)
+        for (int i = 0; i < gs; ++i) add(s.v[lane * gs + i]);
       const uint32_t gkey = score();
       int rank = 0;
-      for (int g = 0; g < n_group; ++g) {
+      for (int g = 0; g < a.n_group; ++g) {
         const uint32_t o = lane_of(gkey, g);
         rank += (o > gkey || (o == gkey && g < lane)) ? 1 : 0;
       }
-      const uint64_t kept = __ballot(lane < n_group && rank < topk_group);
+      const uint64_t kept = __ballot(lane < a.n_group && rank < a.topk_group);
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
         const int e = lane * EPL + j;
-        if (e >= E || !((kept >> (e / gs)) & 1u)) key[j] = 0u;
+        if (e >= a.E || !((kept >> (e / gs)) & 1u)) key[j] = 0u;
       }
     }
   }
@@ -218,7 +274,7 @@ route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const floa
 #pragma unroll
   for (int j = 0; j < EPL; ++j) sel[j] = false;
   int n_sel = 0;
-  for (int r = 0; r < k; ++r) {
+  for (int r = 0; r < a.k; ++r) {
     uint32_t mine = key[0];
 #pragma unroll
     for (int j = 1; j < EPL; ++j) mine = max(mine, key[j]);
@@ -242,20 +298,254 @@ route_topk_kernel(const void* __restrict__ logits, size_t row_stride, const floa
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     if (sel[j]) {
-      s_sel[wave][pos] = s[j];
-      s_id[wave][pos] = lane * EPL + j;
+      s.sel[pos] = sc[j];
+      s.id[pos] = lane * EPL + j;
       ++pos;
     }
   }
-  __syncthreads();
+  wave_fence();
   float sum = 0.0f;  // in ascending expert order
-  for (int r = 0; r < n_sel; ++r) sum += s_sel[wave][r];
+  for (int r = 0; r < n_sel; ++r) sum += s.sel[r];
   sum += 1e-20f;
-  if (active && lane < k) {
+  if (lane < a.k) {
     const bool there = lane < n_sel;
-    const float p = there ? s_sel[wave][lane] : 0.0f;
-    weights[(size_t)t * k + lane] = (renormalize ? __fdiv_rn(p, sum) : p) * scale;
-    ids[(size_t)t * k + lane] = there ? s_id[wave][lane] : -1;
+    const float p = there ? s.sel[lane] : 0.0f;
+    a.weights[(size_t)t * a.k + lane] = (a.renormalize ? __fdiv_rn(p, sum) : p) * a.scale;
+    a.ids[(size_t)t * a.k + lane] = there ? s.id[lane] : -1;
+  }
+}
+
+template <int EPL, int DT, bool SOFTMAX>
+__global__ void __launch_bounds__(64 * WAVES)
+route_topk_kernel(RouteArgs a) {
+  __shared__ RouteLds<EPL> s[WAVES];
+  const int wave = threadIdx.x >> 6, t = blockIdx.x * WAVES + wave;
+  if (t < a.T) route_token<EPL, DT, SOFTMAX>(a, t, s[wave]);
+}
+
+// ---------------------------------------------------------------------------
+// Many tokens: four per wave, 16 lanes each, P experts a lane, the same scores and picks.
+// One token per wave spends most of its instructions on wave-wide maxima of mostly idle
+// lanes; here a lane sorts its experts once and a round of the selection is a row's
+// maximum (four DPP moves for four tokens) and a pop of the winner's list.  Ties, which
+// go to the lower expert, and groups that tie are told by counts and take a longer way.
+// From T = 4096 on, where it takes less; us, one token a wave / four:
+//   256 experts in 8 groups, sigmoid  T=2048 6.0 / 7.3, 4096 8.2 / 7.4, 16384 22.6 / 16.9
+//   160 in 8, softmax, bf16           T=2048 6.7 / 8.7, 4096 9.3 / 9.0, 16384 25.8 / 16.8
+//   64, softmax, bf16                 T=2048 3.5 / 4.0, 4096 4.4 / 4.1, 16384 10.4 / 7.0
+// What bounds it is the vector unit: about 20 f64 instructions a score, 10 for the
+// division, 20 a score for the selection; 17 MB of logits would take 3.4 us.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void order(uint32_t& a, uint32_t& b) {  // a >= b
+  const uint32_t hi = max(a, b), lo = min(a, b);
+  a = hi;
+  b = lo;
+}
+__device__ __forceinline__ void sort4(uint32_t* r) {
+  order(r[0], r[1]); order(r[2], r[3]); order(r[0], r[2]); order(r[1], r[3]); order(r[1], r[2]);
+}
+__device__ __forceinline__ void sort8(uint32_t* r) {  // odd-even merge sort
+  sort4(r);
+  sort4(r + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) order(r[i], r[i + 4]);
+  order(r[2], r[4]); order(r[3], r[5]);
+  order(r[1], r[2]); order(r[3], r[4]); order(r[5], r[6]);
+}
+// Row-wide (16 lanes) reductions, the result in every lane of the row.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  return dpp_max<DPP_MIRROR>(dpp_max<DPP_HALF_MIRROR>(dpp_max<DPP_XOR2>(dpp_max<DPP_XOR1>(x))));
+}
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, dpp<DPP_XOR1>(x));
+  x = fmaxf(x, dpp<DPP_XOR2>(x));
+  x = fmaxf(x, dpp<DPP_HALF_MIRROR>(x));
+  return fmaxf(x, dpp<DPP_MIRROR>(x));
+}
+template <class N>
+__device__ __forceinline__ N row_sum(N x) {
+  x += dpp<DPP_XOR1>(x);
+  x += dpp<DPP_XOR2>(x);
+  x += dpp<DPP_HALF_MIRROR>(x);
+  return x + dpp<DPP_MIRROR>(x);
+}
+template <int N>
+__device__ __forceinline__ int row_shr(int x) {  // lane i: lane i - N's, 0 below
+  return __builtin_amdgcn_update_dpp(0, x, 0x110 + N, 0xF, 0xF, false);
+}
+template <int R>
+__device__ __forceinline__ uint32_t row_ror(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + R, 0xF, 0xF, false);
+}
+// Lanes of the row with a larger key, and with TIES those with an equal one below this.
+template <bool TIES, int R = 1>
+__device__ __forceinline__ int lanes_above(uint32_t key, uint32_t sub) {
+  if constexpr (R == 16) {
+    return 0;
+  } else {
+    // Both moves before any branch: a lane that is switched off has nothing to move.
+    const uint32_t o = row_ror<R>(key), o_sub = TIES ? row_ror<R>(sub) : 0u;
+    const bool above = (o > key) | (TIES & (o == key) & (o_sub < sub));
+    return (above ? 1 : 0) + lanes_above<TIES, R + 1>(key, sub);
+  }
+}
+// Sum of the lanes below in the row.
+__device__ __forceinline__ int row_below(int x) {
+  int s = x;
+  s += row_shr<1>(s);
+  s += row_shr<2>(s);
+  s += row_shr<4>(s);
+  s += row_shr<8>(s);
+  return s - x;
+}
+
+constexpr int ROWS_MAX_K = 8, ROWS_MIN_T = 4096;
+template <int P, int DT, bool SOFTMAX>
+__global__ void __launch_bounds__(64 * WAVES)
+route_rows_kernel(RouteArgs a) {
+  constexpr int LIST = P < ROWS_MAX_K ? P : ROWS_MAX_K;
+  __shared__ int s_id[WAVES][4][ROWS_MAX_K];
+  __shared__ float s_sel[WAVES][4][ROWS_MAX_K];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane >> 4, sub = lane & 15;
+  const int t0 = (blockIdx.x * WAVES + wave) * 4;
+  if (t0 >= a.T) return;  // uniform
+  const int t = min(t0 + row, a.T - 1), per = (a.E + 15) >> 4, e0 = sub * per;
+  const size_t at = (size_t)t * a.row_stride;
+  float x[P], v[P];
+  if (a.vec) {
+    load_all<DT, P>(a.logits, at + e0, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) x[j] = j < per && e0 + j < a.E ? load_as_f32<DT>(a.logits, at + e0 + j) : -INFINITY;
+  }
+  float m = -INFINITY;
+  double inv = 0.0;
+  if constexpr (SOFTMAX) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) m = fmaxf(m, x[j]);
+    m = row_max(m);
+    double ex[P], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      ex[j] = x[j] > -INFINITY ? exp64_below(x[j], m) : 0.0;
+      sum += ex[j];
+    }
+    sum = row_sum(sum);
+    inv = sum > 0.0 ? 1.0 / sum : 0.0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) v[j] = (float)(ex[j] * inv);
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) v[j] = sigmoid(x[j]);
+  }
+  if (a.bias) {
+    if (a.vec) {
+      float b[P];
+      load_all<DT_F32, P>(a.bias, e0, b);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[j] += b[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        if (j < per && e0 + j < a.E) v[j] += a.bias[e0 + j];
+    }
+  }
+  uint32_t key[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) key[j] = x[j] > -INFINITY ? open_key(v[j]) : 0u;
+  if (a.n_group > 1) {
+    const int lpg = a.lanes_per_group;
+    float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const float y = key[j] ? v[j] : -INFINITY;
+      m2 = fmaxf(m2, fminf(m1, y));
+      m1 = fmaxf(m1, y);
+    }
+    auto merge = [&](float o1, float o2) {
+      m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+      m1 = fmaxf(m1, o1);
+    };
+    if (lpg > 1) merge(dpp<DPP_XOR1>(m1), dpp<DPP_XOR1>(m2));
+    if (lpg > 2) merge(dpp<DPP_XOR2>(m1), dpp<DPP_XOR2>(m2));
+    if (lpg > 4) merge(dpp<DPP_HALF_MIRROR>(m1), dpp<DPP_HALF_MIRROR>(m2));
+    const uint32_t score = open_key((a.group_top == 2 && m2 > -INFINITY) ? m1 + m2 : m1);
+    const int most = a.topk_group * lpg;
+    bool kept = lanes_above<false>(score, sub) < most;
+    // Groups that tie for the last place are all kept so far.
+    if (__any(row_sum(kept && score ? 1 : 0) > most)) kept = lanes_above<true>(score, sub) < most;
+#pragma unroll
+    for (int j = 0; j < P; ++j) key[j] = kept ? key[j] : 0u;
+  }
+  // The k-th largest: every lane's largest in order, then k times the row's largest head.
+  uint32_t r[P < 8 ? 8 : P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) r[j] = key[j];
+  if constexpr (P == 4) {
+    sort4(r);
+  } else {
+    sort8(r);
+  }
+  if constexpr (P == 16) {
+    sort8(r + 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = max(r[i], r[15 - i]);  // the 8 largest, a bitonic sequence
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(i & d)) order(r[i], r[i + d]);
+  }
+  uint32_t kth = 0;
+#pragma unroll
+  for (int i = 0; i < ROWS_MAX_K; ++i) {
+    if (i < a.k) {
+      kth = row_max(r[0]);
+      const uint32_t heads = (uint32_t)(__ballot(r[0] == kth) >> (row * 16)) & 0xFFFFu;
+      const bool pop = (heads & -heads) == 1u << sub;  // the first of the lanes that have it
+      // The empty asm keeps the list in its registers: the compiler would turn the moves
+      // into a search for the r[pops so far], 16 comparisons a round.
+#pragma unroll
+      for (int j = 0; j < LIST; ++j)
+        if (j < ROWS_MAX_K - i) {  // as far as the rounds to come reach
+          r[j] = pop ? (j + 1 < LIST ? r[j + 1] : 0u) : r[j];
+          __asm__("" : "+v"(r[j]));
+        }
+    }
+  }
+  uint32_t mask = 0;  // the picks
+#pragma unroll
+  for (int j = 0; j < P; ++j) mask |= (key[j] >= kth && key[j] ? 1u : 0u) << j;
+  int n = row_sum((int)__popc(mask));
+  if (__any(n > a.k)) {  // equals of the k-th are too many: the lower ones stay
+    uint32_t equal = 0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) equal |= (key[j] == kth && key[j] ? 1u : 0u) << j;
+    const int n_equal = row_sum((int)__popc(equal)), room = a.k - (n - n_equal);
+    int left = room - row_below((int)__popc(equal));
+    mask &= ~equal;
+    for (; equal && left > 0; equal &= equal - 1, --left) mask |= equal & -equal;
+    n = row_sum((int)__popc(mask));
+  }
+  int pos = row_below((int)__popc(mask));
+  for (; mask; mask &= mask - 1) s_id[wave][row][pos++] = e0 + __builtin_ctz(mask);
+  wave_fence();
+  const int id = sub < n ? s_id[wave][row][sub] : -1;  // n <= k <= 8
+  float p = 0.0f;
+  if (id >= 0) {
+    const float xi = load_as_f32<DT>(a.logits, at + id);
+    if constexpr (SOFTMAX) p = (float)(exp64_below(xi, m) * inv);
+    else p = sigmoid(xi);
+  }
+  if (sub < ROWS_MAX_K) s_sel[wave][row][sub] = p;
+  wave_fence();
+  float total = 0.0f;  // in ascending expert order
+#pragma unroll
+  for (int i = 0; i < ROWS_MAX_K; ++i) total += s_sel[wave][row][i];
+  total += 1e-20f;
+  if (t0 + row < a.T && sub < a.k) {
+    a.weights[(size_t)t * a.k + sub] = (a.renormalize ? __fdiv_rn(p, total) : p) * a.scale;
+    a.ids[(size_t)t * a.k + sub] = id;
   }
 }
 
@@ -283,7 +573,7 @@ route_topk_backward_kernel(const float* __restrict__ grad, const void* __restric
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      s[j] = x[j] > -INFINITY ? exp_below<float>(x[j], m) : 0.0f;
+      s[j] = x[j] > -INFINITY ? exp32_below(x[j], m) : 0.0f;
       sum += s[j];
     }
     sum = wave_sum(sum);
@@ -356,17 +646,35 @@ hipError_t dispatch(int E, int dtype, int softmax, F&& f) {
 
 }  // namespace
 
+// Lanes of `per` experts that make up a group, if they are a power of two of whole
+// lanes, at most `most`; else 0.
+static int whole_lanes(int group, int per, int most) {
+  const int lanes = group / per;
+  return group % per == 0 && lanes <= most && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+}
+
 hipError_t launch_route_topk(const void* logits, int dtype, size_t row_stride, const float* bias, int T, int E, int k,
                              int softmax, int n_group, int topk_group, int group_top, int renormalize, float scale,
                              float* weights, int32_t* ids, hipStream_t stream) {
+  RouteArgs a = {logits, row_stride, bias, T, E, k, n_group, 0, topk_group, group_top, renormalize, 0, scale, weights, ids};
+  const int per = (E + 15) / 16, rows_lanes = n_group > 1 ? whole_lanes(E / n_group, per, 8) : 1;
+  if (T >= ROWS_MIN_T && E <= 256 && k <= ROWS_MAX_K && rows_lanes > 0) {
+    a.lanes_per_group = rows_lanes;
+    const size_t size = dtype == DT_F32 ? 4 : 2;  // loads of 4 elements
+    a.vec = (E == 64 || E == 128 || E == 256) && row_stride % 4 == 0 && (uintptr_t)logits % (4 * size) == 0 &&
+            (uintptr_t)bias % 16 == 0;
+    return dispatch(E, dtype, softmax, [&](auto epl, auto dt, auto sm) {
+      constexpr int EPL = decltype(epl)::value;
+      if constexpr (EPL <= 4)
+        route_rows_kernel<4 * EPL, decltype(dt)::value, decltype(sm)::value>
+            <<<(T + 4 * WAVES - 1) / (4 * WAVES), 64 * WAVES, 0, stream>>>(a);
+    });
+  }
   return dispatch(E, dtype, softmax, [&](auto epl, auto dt, auto sm) {
     constexpr int EPL = decltype(epl)::value;
-    const int gs = E / n_group, lanes = gs / EPL;
-    const bool whole = gs % EPL == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0;
-    route_topk_kernel<decltype(epl)::value, decltype(dt)::value, decltype(sm)::value>
-        <<<(T + WAVES - 1) / WAVES, 64 * WAVES, 0, stream>>>(logits, row_stride, bias, T, E, k, n_group,
-                                                             whole ? lanes : 0, topk_group, group_top, renormalize,
-                                                             scale, weights, ids);
+    a.lanes_per_group = whole_lanes(E / n_group, EPL, 16);
+    route_topk_kernel<EPL, decltype(dt)::value, decltype(sm)::value>
+        <<<(T + WAVES - 1) / WAVES, 64 * WAVES, 0, stream>>>(a);
   });
 }
 

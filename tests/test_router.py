@@ -162,8 +162,48 @@ def test_route_topk(ops, cuda, shape, scoring, kind):
 
 
 @pytest.mark.gpu
-def test_route_topk_equals_the_layers_router(ops, cuda):
-    x = _logits(1000, 256, 21, torch.float32, "plain").to(cuda)
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[0] <= 256 and s[4] <= 8], ids=str)
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("kind", ["plain", "masked", "ties", "far", "near"])
+def test_route_topk_many_tokens(ops, cuda, shape, scoring, kind):
+    """From 4096 tokens on a wave takes four; `near`: rows whose best logits are a few units of the last place apart, and
+    equal ones, around every place of the border."""
+    E, groups, kept, top, k = shape
+    T = 4099
+    for i, (dtype, biases) in enumerate([(torch.float32, ("none", "plain")), (torch.bfloat16, ("none", "closed")),
+                                         (torch.float16, ("plain",))]):
+        x = _logits(T, E, 17 * E + i, torch.float32, "plain" if kind == "near" else kind)
+        if kind == "near":
+            g = torch.Generator().manual_seed(E + i)
+            x = x.abs().neg()
+            x += 3.0 * (torch.rand(T, E, generator=g) < 1.5 * k / E)
+            close = torch.rand(T, E, generator=g) < 2.0 * k / E
+            x = torch.where(close, 1.5 + torch.randint(0, 3, (T, 1), generator=g) * 0.7, x)
+            x = torch.where(close, x * (1 + torch.randint(-3, 4, (T, E), generator=g) * 2.0**-23), x)
+        x = x.to(dtype).to(cuda)
+        for bias in biases:
+            b = _bias(E, E + i, bias)
+            if kind == "near" and b is not None:
+                b = (b * 4).round() / 4
+            _check(ops, x, b, k, scoring, groups, kept, top, bool(i & 1), (1.0, 2.5)[i & 1], cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [4095, 4096, 4097])
+def test_route_topk_many_tokens_large_bias(ops, cuda, T):
+    """Biases that dwarf the scores, of both signs: groups' sums cancel, and v keeps few of the score's digits."""
+    x = _logits(T, 256, T, torch.float32, "plain").to(cuda)
+    for scale in (30.0, 1e4, 1e30):
+        b = _bias(256, 3, "plain") * scale
+        b[7], b[40] = torch.inf, 3e38
+        _check(ops, x, b, 8, "sigmoid", 8, 4, 2, True, 1.0, cuda)
+        _check(ops, x, b, 6, "softmax", 1, 1, 2, False, 1.0, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1000, 6000])
+def test_route_topk_equals_the_layers_router(ops, cuda, T):
+    x = _logits(T, 256, 21, torch.float32, "plain").to(cuda)
     bias = _bias(256, 22, "plain").to(cuda)
     w, ids = ops.route_topk(x, bias, 8, "sigmoid", 8, 4, scale=2.5)
     ref = ops.route(x, bias, 2.5, 0)
@@ -172,6 +212,9 @@ def test_route_topk_equals_the_layers_router(ops, cuda):
 
 @pytest.mark.gpu
 def test_route_topk_strided_and_odd_rows(ops, cuda):
+    many = _logits(4100, 131, 32, torch.float32, "plain").to(cuda)
+    for x in (many[:, :128], many[:, 3:131], many[:, 2:66], many[:1].expand(4100, 131)[:, :64]):
+        _check(ops, x, None, 4, "sigmoid", 4, 2, 2, True, 1.0, cuda)
     wide = _logits(50, 301, 31, torch.bfloat16, "plain").to(cuda)
     for x in (wide[:, 7:167], wide[::3, 1:65], wide[:1].expand(9, 301)[:, :96], wide[10:10, :64]):
         assert x.size(0) < 2 or not x.is_contiguous()
