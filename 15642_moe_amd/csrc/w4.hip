@@ -1303,6 +1303,13 @@ hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, 
   return hipGetLastError();
 }
 
+// Whether a dense product runs in tiles.  A tile launch of few items takes its K loop's
+// time, a stream's time goes with the outputs; us, tiles / streams:
+//   N=4096 K=7168  T=64 24.0 / 12.6, 128 23.9 / 20.7, 192 23.6 / 30.4
+//   N=7168 K=2048  T=33 7.6 / 7.4, 48 7.6 / 8.1, 128 7.8 / 12.8
+//   N=1024 K=1024  T=256 5.2 / 4.6;  N=512 K=7168  T=256 16.7 / 11.8
+static bool linear_in_tiles(int T, int N, int K) { return (size_t)T * N > 300000 + 30 * (size_t)K; }
+
 // Fragments per wave of a tile launch: the fewest whole rounds of workgroups over
 // the CUs, each as long as its fragments and a constant share (weights, barriers).
 static int linear_tile_nc(int T, int tiles, int cus) {
@@ -1326,7 +1333,7 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
                             uint16_t* out, hipStream_t stream) {
   const int tiles = w4_tiles(N), KC = w4_chunks(K);
   const int waves = stream_waves(KC);
-  if (T > 64) {
+  if (linear_in_tiles(T, N, K)) {
     auto tile = [&](auto kernel, int nc) {
       const size_t items = (size_t)((tiles + 15) / 16) * ((T + TILE_COLS * nc - 1) / (TILE_COLS * nc));
       by_grids(items, [&](unsigned grid, int base) {
@@ -1349,6 +1356,16 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
   if (T <= 16) launch(linear_w4_kernel<1, 1>, 1, 1);
   else launch(linear_w4_kernel<2, 2>, 2, 2);
   return hipGetLastError();
+}
+
+// Whether the experts' products run in tiles: from 49 tokens on where a tile per
+// expert fills the CUs, else from 385 on.  Whole call, us, tiles / streams:
+//   7168, 2048, 32 of 256, top 8   even T=32 112 / 111, 64 133 / 142, 128 146 / 160, 512
+//     170 / 252; uneven T=32 53 / 50, 64 57 / 57, 128 61 / 77, 512 93 / 209
+//   2048, 768, 128 of 128, top 8   even T=32 75 / 74, 64 84 / 85, 512 111 / 178
+//   1024, 512, 16 of 64, top 4 (64 items)   even T=64 21 / 18, 256 25 / 22, 512 26 / 26
+static bool experts_in_tiles(const ExpertsW4& a) {
+  return a.T > ((long long)a.e_local * (a.I / BLK) >= device_cus() ? 48 : 384);
 }
 
 size_t experts_w4_workspace(int T, int H, int I, int e_local, int k) {
@@ -1375,7 +1392,7 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
     few_gemm2_kernel<<<a.H / 32, FEW_THREADS, 16 * a.I, stream>>>(a, Cf);
     return hipGetLastError();
   }
-  const bool tile = a.T > 256;
+  const bool tile = experts_in_tiles(a);
   const int fr = a.T <= 16 ? 1 : 2;
   const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus() * (2 / TILE_CW)};
   if (picks <= SORT_SMALL) {

@@ -274,6 +274,28 @@ def test_linear_w4_large(ops, cuda, T, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K", [(65, 7168, 2048), (300, 1301, 384), (700, 530, 1152), (4100, 100, 128), (257, 2064, 640),
+                                   (960, 4096, 128), (1200, 4091, 256), (1900, 4096, 128), (1200, 8192, 128)])
+def test_linear_w4_tiles(ops, cuda, T, N, K):
+    """Sizes that run in tiles: ragged ends of every kind, and of 1 to 5 fragments a wave."""
+    _check_linear(ops, cuda, np.random.default_rng(T + N + K), T, N, K)
+
+
+@pytest.mark.gpu
+def test_linear_w4_same_rows_at_any_batch(ops, cuda):
+    """A NaN row, and rows behind it, leave the others' values alone."""
+    rng = np.random.default_rng(12)
+    xc, xs = _act(rng, 700, 640)
+    xc[333] = 0x7F
+    codes, scales = _matrix(rng, 1040, 640)
+    p = ops.pack_w4(_dev(codes, cuda), _dev(scales, cuda))
+    y = ops.linear_w4(_dev(xc, cuda, F8), _dev(xs, cuda), p)
+    assert torch.isnan(y[333]).all() and torch.isfinite(y[:333]).all() and torch.isfinite(y[334:]).all()
+    few = ops.linear_w4(_dev(xc[325:341], cuda, F8), _dev(np.ascontiguousarray(xs[:, 325:341]), cuda), p)
+    assert torch.isnan(few[8]).all() and torch.isfinite(few[:8]).all() and torch.isfinite(few[9:]).all()
+
+
+@pytest.mark.gpu
 def test_linear_w4_single_elements(ops, cuda):
     """One-hot activations read single weights: the operand layouts and the place of each scale, exactly."""
     rng = np.random.default_rng(8)
@@ -369,7 +391,7 @@ def _wild(rng, T, k, E):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1, 2, 7, 16, 17, 40, 100, 300])
+@pytest.mark.parametrize("T", [1, 2, 7, 16, 17, 40, 100, 300, 400, 1000])
 @pytest.mark.parametrize("hidden,inter,E,k", [(128, 128, 3, 2), (640, 384, 5, 4), (512, 1152, 2, 2)])
 def test_experts_w4(ops, cuda, T, hidden, inter, E, k):
     rng = np.random.default_rng(T + hidden)
@@ -381,7 +403,7 @@ def test_experts_w4(ops, cuda, T, hidden, inter, E, k):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1, 19, 130])
+@pytest.mark.parametrize("T", [1, 19, 130, 450])
 def test_experts_w4_layer_size(ops, cuda, T):
     rng = np.random.default_rng(T)
     case = _experts_case(rng, T, 7168, 2048, 2, 8, lambda r, t, k, e: _even(r, t, k, 4))
@@ -392,7 +414,7 @@ def test_experts_w4_layer_size(ops, cuda, T):
 def test_experts_w4_many_experts_and_picks(ops, cuda):
     """More picks than one workgroup sorts (2048), 1024 experts, up to 64 picks a token."""
     rng = np.random.default_rng(5)
-    for T, E, k in ((130, 1024, 64), (2100, 40, 5), (8193, 3, 1)):
+    for T, E, k in ((40, 1024, 64), (130, 1024, 64), (2100, 40, 5), (8193, 3, 1)):
         case = _experts_case(rng, T, 128, 128, E, k, lambda r, t, kk, e: np.argsort(r.random((t, e)), axis=1)[:, :kk])
         _check_experts(ops, cuda, case, 0)
 
@@ -400,7 +422,7 @@ def test_experts_w4_many_experts_and_picks(ops, cuda):
 @pytest.mark.gpu
 def test_experts_w4_same_result_every_time(ops, cuda):
     rng = np.random.default_rng(6)
-    for T in (9, 700):
+    for T in (3, 9, 30, 700):
         case = _experts_case(rng, T, 256, 256, 4, 4, lambda r, t, k, e: _even(r, t, k, 2))
         first = _run_experts(ops, cuda, case, 0)
         for _ in range(3):
