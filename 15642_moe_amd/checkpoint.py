@@ -211,6 +211,52 @@ def load_moe_layer(path: str | os.PathLike, layer: int, local_expert_offset: int
     return MoELayerWeights(layer, local_expert_offset, w13, w13_scale, w2, w2_scale, routing_bias, router, pack)
 
 
+@dataclass
+class MoELayerWeightsW4:
+    """One layer's local experts in 4 bits: `w13` / `w2` are ops.pack_w4 results, for ops.moe_forward_w4 or
+    ops.experts_w4."""
+
+    layer: int
+    local_expert_offset: int
+    w13: torch.Tensor            # uint8 [E, 256, 14, 4352]
+    w2: torch.Tensor             # uint8 [E, 448, 4, 4352]
+    routing_bias: torch.Tensor   # f32 [256]
+    router_weight: torch.Tensor | None
+
+
+def load_moe_layer_w4(path: str | os.PathLike, layer: int, local_expert_offset: int = 0, n_local: int = MAX_E_LOCAL,
+                      device: str | torch.device = "cuda") -> MoELayerWeightsW4:
+    """Experts local_expert_offset .. +n_local of `layer`, dequantised from their FP8 blocks and requantised to OCP
+    MXFP4 (ops.quantize_w4), each straight into its slot of the packed buffers: the device holds the packed weights and
+    one expert in 32 bits."""
+    from . import ops
+
+    if n_local < 1 or local_expert_offset < 0 or local_expert_offset + n_local > E_GLOBAL:
+        raise ValueError(f"experts {local_expert_offset}..{local_expert_offset + n_local - 1} are not all in 0..255")
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise RuntimeError("4-bit weights need a HIP device (quantisation and packing run on the GPU)")
+    ck = Checkpoint(path)
+    routing_bias = ck.get(bias_key(layer), (E_GLOBAL,), torch.float32).to(dev)
+    router = ck.get(router_key(layer), (E_GLOBAL, H), torch.bfloat16).to(dev) if router_key(layer) in ck else None
+
+    def wide(w, scale):
+        w, scale = w.to(dev).float(), scale.to(dev)
+        rows, cols = scale.shape
+        return w.view(rows, -1, cols, w.shape[1] // cols).mul_(scale[:, None, :, None]).view(w.shape)
+
+    w13 = w2 = None
+    for le in range(n_local):
+        up, gate, down, up_s, gate_s, down_s = _expert_tensors(ck, layer, local_expert_offset + le)
+        p13 = ops.pack_w4(*ops.quantize_w4(torch.cat([wide(up, up_s), wide(gate, gate_s)])))
+        p2 = ops.pack_w4(*ops.quantize_w4(wide(down, down_s)))
+        if le == 0:
+            w13, w2 = (torch.empty((n_local, *p.shape), dtype=torch.uint8, device=dev) for p in (p13, p2))
+        w13[le], w2[le] = p13, p2
+    torch.cuda.current_stream(dev).synchronize()
+    return MoELayerWeightsW4(layer, local_expert_offset, w13, w2, routing_bias, router)
+
+
 def save_moe_layer(path: str | os.PathLike, layer: int, experts: dict, routing_bias: torch.Tensor,
                    router_weight: torch.Tensor | None = None, shards: int = 1) -> None:
     """Write expert tensors in the checkpoint layout (for tests and for

@@ -23,7 +23,9 @@ from .geometry import (
     I_BLOCKS,
     I_DIM,
     MAX_E_LOCAL,
+    N_GROUP,
     TOP_K,
+    TOPK_GROUP,
     W13_PACKED_SHAPE,
     W2_PACKED_SHAPE,
 )
@@ -518,6 +520,15 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     _call("experts_w4", lib.moe_experts_w4, dev, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
           ids.data_ptr(), weights.data_ptr(), T, K, inter, E, k, local_offset, ws.data_ptr(), ws_bytes, out.data_ptr())
     return out
+
+
+def moe_forward_w4(hidden, hidden_scale, w13: torch.Tensor, w2: torch.Tensor, logits, bias, rsf: float,
+                   local_offset: int) -> torch.Tensor:
+    """moe_forward with 4-bit weights: the layer's router (no-aux-loss, 8 groups, top 4, top 8 of 256) and experts_w4.
+    Arguments as moe_forward's, with pack_w4 results in the place of the packed FP8 weights and their scales."""
+    _check(logits.dim() == 2 and logits.size(1) == E_GLOBAL, "logits must be [T, 256]")
+    weights, ids = _route_topk(logits, bias, TOP_K, "sigmoid", N_GROUP, TOPK_GROUP, 2, True, rsf)
+    return experts_w4(hidden, hidden_scale, w13, w2, ids, weights, local_offset)
 
 
 # --------------------------------------------------------------------------- inspection

@@ -4,6 +4,7 @@ which derives the bounds beside its formulas."""
 from __future__ import annotations
 
 import ctypes
+import importlib
 
 import numpy as np
 import pytest
@@ -11,6 +12,7 @@ import torch
 
 from oracle import router as orouter
 from oracle import w4 as oracle
+from oracle.numerics import e4m3_encode
 
 
 F8 = torch.float8_e4m3fn
@@ -545,3 +547,77 @@ def test_w4_two_streams(ops, cuda):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 2])
+
+
+# ------------------------------------------------------------------------------------------------ the layer and its loader
+def test_checkpoint_w4_refusals(tmp_path):
+    ck = importlib.import_module("15642_moe_amd.checkpoint")
+    with pytest.raises(ValueError, match="0..255"):
+        ck.load_moe_layer_w4(tmp_path, 0, 250, 10)
+    with pytest.raises(ValueError, match="0..255"):
+        ck.load_moe_layer_w4(tmp_path, 0, 0, 0)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ck.load_moe_layer_w4(tmp_path, 0, 0, 1, device="cpu")
+
+
+@pytest.mark.gpu
+def test_checkpoint_w4(tmp_path, ops, cuda):
+    """A layer's FP8 experts from a checkpoint, in 4 bits: some rows of every part against the oracle's quantisation."""
+    from oracle.numerics import E4M3_TABLE
+
+    ck = importlib.import_module("15642_moe_amd.checkpoint")
+    rng = np.random.default_rng(20)
+
+    def expert():
+        w = [torch.from_numpy(e4m3_encode(rng.standard_normal(s).astype(np.float32))).view(F8) for s in ((4096, 7168), (7168, 2048))]
+        s = [torch.from_numpy(rng.uniform(1e-3, 1e-2, n).astype(np.float32)) for n in ((32, 56), (56, 16))]
+        return w[0], s[0], w[1], s[1]
+
+    experts = {7: expert(), 8: expert()}
+    bias = torch.linspace(-1, 1, 256)
+    ck.save_moe_layer(tmp_path, 3, experts, bias)
+    layer = ck.load_moe_layer_w4(tmp_path, 3, 7, 2, device=cuda)
+    assert layer.router_weight is None and torch.equal(layer.routing_bias.cpu(), bias)
+    for e in (0, 1):
+        for packed, w, s, N, K in ((layer.w13[e], *experts[7 + e][:2], 4096, 7168), (layer.w2[e], *experts[7 + e][2:], 7168, 2048)):
+            codes, scales = (t.cpu().numpy() for t in ops.unpack_w4(packed, N, K))
+            for row in (0, 127, 128, 2047, 2048, N - 1):
+                wide = E4M3_TABLE[w[row].view(torch.uint8).numpy()].astype(np.float32) * np.repeat(s[row // 128].numpy(), 128)
+                want = oracle.quantize(wide[None])
+                assert np.array_equal(codes[row], want[0][0]) and np.array_equal(scales[row], want[1][0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 33, 300])
+def test_moe_forward_w4_equals_fp8(ops, cuda, T):
+    """4-bit weights whose scales are equal over 128 x 128 blocks are e4m3 weights with those block scales, exactly: both
+    layers' results lie within the oracle's bounds of one exact result, so within two of each other."""
+    rng = np.random.default_rng(T)
+    E, off = 2, 32
+
+    def pair(N, K):
+        codes = _codes(rng, E, N, K // 2)
+        block = rng.integers(116, 120, size=(E, N // 128, K // 128), dtype=np.uint8)
+        scales = np.repeat(np.repeat(block, 128, 1), 4, 2)
+        fp8 = e4m3_encode(oracle.E2M1.astype(np.float32))
+        w8 = np.stack([fp8[codes & 15], fp8[codes >> 4]], -1).reshape(E, N, K)
+        packed = ops.pack_w4(_dev(codes, cuda), _dev(np.ascontiguousarray(scales), cuda))
+        return packed, _dev(w8, cuda, F8), _dev(np.ldexp(1.0, block.astype(np.int32) - 127).astype(np.float32), cuda), (codes, scales)
+
+    p13, f13, s13, c13 = pair(4096, 7168)
+    p2, f2, s2, c2 = pair(7168, 2048)
+    xc, xs = _act(rng, T, 7168)
+    x, s = _dev(xc, cuda, F8), _dev(xs, cuda)
+    logits = torch.from_numpy(rng.standard_normal((T, 256)).astype(np.float32)).to(cuda)
+    bias = torch.zeros(256, device=cuda)
+    bias[off] = 2.0
+    y4 = ops.moe_forward_w4(x, s, p13, p2, logits, bias, 2.5, off)
+    y8 = ops.moe_forward(x, s, ops.pack_w13(f13), s13, ops.pack_w2(f2), s2, logits, bias, 2.5, off)
+    n = slice(0, 20)
+    weights, ids = orouter.route(logits.cpu().numpy(), bias.cpu().numpy(), 8, "sigmoid", 8, 4, 2, True, 2.5)
+    want, bound = oracle.experts(xc[n], np.ascontiguousarray(xs[:, n]), oracle.decode(*c13), oracle.decode(*c2), ids[n],
+                                 weights[n], off)
+    a, b = (t.double().cpu().numpy() for t in (y4, y8))
+    assert (np.abs(a[n] - want) <= bound).all()
+    assert (np.abs(a[n] - b[n]) <= 2 * bound).all()
+    assert np.linalg.norm(a - b) <= 0.01 * np.linalg.norm(b) and np.linalg.norm(b) > 0
