@@ -43,6 +43,19 @@ __device__ __forceinline__ void store_f32_as(void* base, size_t i, float v) {
   else static_cast<_Float16*>(base)[i] = (_Float16)v;
 }
 
+template <int DT>
+__device__ __forceinline__ void store_4(void* base, size_t i, const float (&v)[4]) {  // aligned to the four
+  if constexpr (DT == DT_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) store_f32_as<DT>(h, q, v[q]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) =
+        make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+  }
+}
+
 // P consecutive elements, in loads of up to 16 bytes (the pointer aligned to them).
 template <int DT, int P>
 __device__ __forceinline__ void load_all(const void* base, size_t i, float (&x)[P]) {
@@ -549,78 +562,124 @@ route_rows_kernel(RouteArgs a) {
   }
 }
 
-template <int EPL, int DT, bool SOFTMAX>
+// ---------------------------------------------------------------------------
+// The gradient: L = 16 or 64 lanes a token, a lane the experts 4 (i L + l) .. +4 of each
+// piece i, so that loads and stores are whole lines.  The picks' gradients, a lane each,
+// go to the token's row in LDS; with sigmoid they are the result (only the picks' logits
+// are read), with softmax each expert's share of the normaliser is added to them.
+// ---------------------------------------------------------------------------
+template <int L, class N>
+__device__ __forceinline__ N lanes_sum(N x) {
+  if constexpr (L == 16) return row_sum(x);
+  else return wave_sum(x);
+}
+template <int L, int P, int DT, bool SOFTMAX>
 __global__ void __launch_bounds__(64 * WAVES)
 route_topk_backward_kernel(const float* __restrict__ grad, const void* __restrict__ logits, size_t row_stride,
                            const int32_t* __restrict__ ids, int T, int E, int k, int renormalize, float scale,
-                           void* __restrict__ out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x * WAVES + wave;
-  if (t >= T) return;
-  const size_t row = (size_t)t * row_stride;
-  float x[EPL], s[EPL], slope[EPL], d[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane * EPL + j;
-    x[j] = e < E ? load_as_f32<DT>(logits, row + e) : -INFINITY;
-    d[j] = 0.0f;
-  }
+                           int vec, void* __restrict__ out) {
+  constexpr int TOKENS = 64 / L;  // a wave's
+  __shared__ __align__(16) float s_d[WAVES][TOKENS][L * P];
+  __shared__ int2 s_pick[WAVES][TOKENS][L];  // id, gradient
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane / L, sub = lane % L;
+  const int t0 = (blockIdx.x * WAVES + wave) * TOKENS;
+  if (t0 >= T) return;  // uniform
+  const int t = min(t0 + row, T - 1);
+  const size_t at = (size_t)t * row_stride;
+  float* d = s_d[wave][row];
+  int2* picks = s_pick[wave][row];
+  // Lane r < k: pick r.
+  int id = sub < k ? ids[(size_t)t * k + sub] : -1;
+  if (id >= E) id = -1;
+  const float g = id >= 0 ? grad[(size_t)t * k + sub] : 0.0f;
+  float s[P], m = -INFINITY, inv = 0.0f;
   if constexpr (SOFTMAX) {
-    float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) m = fmaxf(m, x[j]);
-    m = wave_max(m);
+    for (int i = 0; i < P / 4; ++i) {
+      const int e = 4 * (i * L + sub);
+      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (vec) {
+        if (e < E) load_all<DT, 4>(logits, at + e, x);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (e + q < E) x[q] = load_as_f32<DT>(logits, at + e + q);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[i * 4 + q] = x[q];
+    }
+  }
+  const float xp = id >= 0 ? load_as_f32<DT>(logits, at + id) : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < P / 4; ++i)
+    if (i * 4 * L < E) *reinterpret_cast<float4*>(d + 4 * (i * L + sub)) = make_float4(0.f, 0.f, 0.f, 0.f);
+  float p, slope = 0.0f;
+  if constexpr (SOFTMAX) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) m = fmaxf(m, s[j]);
+    if constexpr (L == 16) m = row_max(m);
+    else m = wave_max(m);
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      s[j] = x[j] > -INFINITY ? exp32_below(x[j], m) : 0.0f;
-      sum += s[j];
-    }
-    sum = wave_sum(sum);
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    for (int i = 0; i < P / 4; ++i) {
+      if (i * 4 * L < E) {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] *= inv;
+        for (int j = 4 * i; j < 4 * i + 4; ++j) {
+          s[j] = s[j] > -INFINITY ? exp32_below(s[j], m) : 0.0f;
+          sum += s[j];
+        }
+      }
+    }
+    sum = lanes_sum<L>(sum);
+    inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    p = xp > -INFINITY ? exp32_below(xp, m) * inv : 0.0f;
   } else {
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      // both factors from exp(-|x|): 1 - s keeps its digits where s is near 1
-      const float q = x[j] > -INFINITY ? expf(-fabsf(x[j])) : 0.0f;
-      const float a = 1.0f / (1.0f + q), b = q * a;
-      s[j] = x[j] >= 0.0f ? a : b;
-      slope[j] = a * b;
-    }
-  }
-  // Lane r < k: pick r, its score and weight gradient.
-  const int id = lane < k ? ids[(size_t)t * k + lane] : -1;
-  const bool there = id >= 0 && id < E;
-  const float g = there ? grad[(size_t)t * k + lane] : 0.0f;
-  float p = 0.0f;
-  {
-    const int at = there ? id / EPL : 0, sub = there ? id % EPL : 0;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const float o = __shfl(s[j], at);
-      p = sub == j ? o : p;
-    }
-    p = there ? p : 0.0f;
+    // both factors from exp(-|x|): 1 - s keeps its digits where s is near 1
+    const float q = xp > -INFINITY ? expf(-fabsf(xp)) : 0.0f;
+    const float a = 1.0f / (1.0f + q), b = q * a;
+    p = xp >= 0.0f ? a : b;
+    slope = a * b;
   }
   float ds = scale * g;
   if (renormalize) {
-    const float inv = 1.0f / (wave_sum(p) + 1e-20f);
-    ds = scale * ((g - wave_sum(g * p) * inv) * inv);
-    ds = there ? ds : 0.0f;
+    const float inv_p = 1.0f / (lanes_sum<L>(p) + 1e-20f);
+    const float part = lanes_sum<L>(g * p) * inv_p;  // by all lanes: before the choice
+    ds = id >= 0 ? scale * ((g - part) * inv_p) : 0.0f;
   }
-  for (int r = 0; r < k; ++r) {
-    const int e = __builtin_amdgcn_readlane(there ? id : -1, r) - lane * EPL;
-    const float dr = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(ds), r));
+  const float mean = SOFTMAX ? lanes_sum<L>(ds * p) : 0.0f;
+  const float mine = SOFTMAX ? ds : ds * slope;
+  picks[sub] = make_int2(id, __float_as_int(mine));
+  wave_fence();
+  // A pick that stands in several slots: each of them writes the sum over all, in their
+  // order.  (Slots up to the next multiple of 8 are there, and empty.)
+  float all = 0.0f;
+  for (int r0 = 0; r0 < k; r0 += 8) {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) d[j] += e == j ? dr : 0.0f;
+    for (int r = 0; r < 8; ++r) {
+      const int2 o = picks[r0 + r];
+      all += o.x == id ? __int_as_float(o.y) : 0.0f;
+    }
   }
-  const float mean = SOFTMAX ? wave_sum(ds * p) : 0.0f;
+  if (id >= 0) d[id] = all;
+  wave_fence();
+  if (t0 + row >= T) return;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane * EPL + j;
-    if (e < E) store_f32_as<DT>(out, (size_t)t * E + e, SOFTMAX ? s[j] * (d[j] - mean) : d[j] * slope[j]);
+  for (int i = 0; i < P / 4; ++i) {
+    const int e = 4 * (i * L + sub);
+    if (e >= E) break;
+    const float4 u = *reinterpret_cast<const float4*>(d + e);
+    float y[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (SOFTMAX) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y[q] = s[i * 4 + q] * inv * (y[q] - mean);
+    }
+    if (vec) {
+      store_4<DT>(out, (size_t)t * E + e, y);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (e + q < E) store_f32_as<DT>(out, (size_t)t * E + e + q, y[q]);
+    }
   }
 }
 
@@ -681,10 +740,27 @@ hipError_t launch_route_topk(const void* logits, int dtype, size_t row_stride, c
 hipError_t launch_route_topk_backward(const float* grad, const void* logits, int dtype, size_t row_stride,
                                       const int32_t* ids, int T, int E, int k, int softmax, int renormalize,
                                       float scale, void* grad_logits, hipStream_t stream) {
+  const size_t size = dtype == DT_F32 ? 4 : 2;  // loads and stores of 4 elements
+  const int vec = E % 4 == 0 && row_stride % 4 == 0 && (uintptr_t)logits % (4 * size) == 0;
+  // 16 lanes a token where there are tokens enough; us, 64 lanes / 16:
+  //   160 experts, softmax, bf16  T=2048 3.2 / 4.1, 4096 4.0 / 4.3, 8192 5.5 / 4.7, 16384 8.8 / 6.4
+  //   100, softmax, f32           T=2048 3.3 / 3.5, 4096 4.2 / 3.7, 16384 9.5 / 5.5
+  //   60, softmax, bf16           T=1024 3.1 / 3.0, 4096 4.2 / 3.1, 16384 9.3 / 4.1
+  //   256, sigmoid, f32           T=2048 2.8 / 3.0, 16384 7.0 / 7.0: always 64
+  // What bounds it at T = 16384 is the memory's latency and 16 exponentials a lane; 160
+  // experts' 10.5 MB in and out would take 2.0 us.
+  const bool rows = E <= 256 && k <= 16 && T >= 32 * E;
   return dispatch(E, dtype, softmax, [&](auto epl, auto dt, auto sm) {
-    route_topk_backward_kernel<decltype(epl)::value, decltype(dt)::value, decltype(sm)::value>
-        <<<(T + WAVES - 1) / WAVES, 64 * WAVES, 0, stream>>>(grad, logits, row_stride, ids, T, E, k, renormalize,
-                                                             scale, grad_logits);
+    constexpr int EPL = decltype(epl)::value, DT = decltype(dt)::value;
+    constexpr bool SOFTMAX = decltype(sm)::value;
+    auto launch = [&](auto kernel, int tokens) {
+      kernel<<<(T + tokens - 1) / tokens, 64 * WAVES, 0, stream>>>(grad, logits, row_stride, ids, T, E, k, renormalize,
+                                                                   scale, vec, grad_logits);
+    };
+    if constexpr (EPL <= 4 && SOFTMAX) {
+      if (rows) return launch(route_topk_backward_kernel<16, 4 * EPL, DT, SOFTMAX>, 4 * WAVES);
+    }
+    launch(route_topk_backward_kernel<64, EPL < 4 ? 4 : EPL, DT, SOFTMAX>, WAVES);
   });
 }
 

@@ -336,3 +336,23 @@ def test_route_topk_streams_and_graph(ops, cuda):
         we, idse = ops.route_topk(x, bias, 8, "sigmoid", 8, 4)
         assert torch.equal(w, we) and torch.equal(ids, idse)
         assert torch.equal(d, ops.route_topk_backward(g, x, idse))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k,dtype", [(60, 4, torch.bfloat16), (64, 16, torch.float16), (100, 8, torch.float32),
+                                       (129, 16, torch.bfloat16), (256, 8, torch.float32), (64, 17, torch.float32)])
+def test_route_topk_backward_many_tokens(ops, cuda, E, k, dtype):
+    """Either side of the size from which a token takes 16 lanes, with repeated and empty picks, rows apart."""
+    for T in (32 * E - 1, 32 * E, 32 * E + 3):
+        rng = np.random.default_rng(T + k)
+        x = torch.from_numpy(rng.standard_normal((T, E + 4)).astype(np.float32)).to(cuda, dtype)[:, :E]
+        ids = torch.from_numpy(rng.integers(-1, E + 1, size=(T, k)).astype(np.int32)).to(cuda)
+        ids[::3] = ids[::3, :1]
+        g = torch.from_numpy(rng.standard_normal((T, k)).astype(np.float32)).to(cuda)
+        rows = torch.cat([torch.arange(40), torch.arange(T - 40, T)]).to(cuda)
+        for renormalize in (False, True):
+            got = ops.route_topk_backward(g, x, ids, "softmax", renormalize, 2.5)
+            one = ops.route_topk_backward(g[rows], x[rows], ids[rows], "softmax", renormalize, 2.5)
+            _check_grad(got[rows], g[rows], x[rows], ids[rows], "softmax", renormalize, 2.5)
+            _check_grad(one, g[rows], x[rows], ids[rows], "softmax", renormalize, 2.5)
+            assert torch.equal(got, ops.route_topk_backward(g, x, ids, "softmax", renormalize, 2.5))
