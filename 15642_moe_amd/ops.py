@@ -359,7 +359,9 @@ def route_topk(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, scor
 
     An expert whose logit (or logit's score + bias) is -inf or NaN is never picked; a slot that no expert fills holds
     id -1 and weight 0.  The weights are differentiable in the logits; the bias only balances load and takes no
-    gradient.  `experts_w4` takes the result as it is."""
+    gradient.  `experts_w4` takes the result as it is (under no_grad, where the logits are a parameter's).  A captured
+    backward pass calls for what every captured one does: no eager graph of the same leaves alive beside it;
+    route_topk_backward has no such condition."""
     topk_group = n_group if topk_group is None else topk_group
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteTopK.apply(logits, None if bias is None else bias.detach(), top_k, scoring, n_group, topk_group,
@@ -498,7 +500,7 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     (rows [0, inter) multiply, SiLU takes rows [inter, 2 * inter), as in moe_forward) and [e_local, hidden, inter]; ids
     int32 [T, top_k] and weights f32 [T, top_k] as route_topk gives them.  Picks outside [local_offset, local_offset +
     e_local) are another rank's, or none, and add nothing; a token without local picks gets zeros.  hidden and inter
-    are multiples of 128."""
+    are multiples of 128.  For serving: it has no gradient, and refuses weights that would lose theirs."""
     T, K, dev = _check_act(x, x_scale)
     _check(w13.dim() == 4 and w2.dim() == 4, "w13 and w2 must be pack_w4 results [e_local, row tiles, chunks, 4352]")
     E, inter = int(w13.size(0)), 8 * int(w13.size(1))
@@ -512,6 +514,8 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
            "weights must be float32 [T, top_k] contiguous")
     _require_device("ids", ids, dev)
     _require_device("weights", weights, dev)
+    _check(not (weights.requires_grad and torch.is_grad_enabled()),
+           "experts_w4 has no gradient: call it under torch.no_grad(), or with weights.detach()")
     k = int(ids.size(1))
     lib = capi.load()
     ws_bytes = int(lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k))

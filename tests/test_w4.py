@@ -621,3 +621,18 @@ def test_moe_forward_w4_equals_fp8(ops, cuda, T):
     assert (np.abs(a[n] - want) <= bound).all()
     assert (np.abs(a[n] - b[n]) <= 2 * bound).all()
     assert np.linalg.norm(a - b) <= 0.01 * np.linalg.norm(b) and np.linalg.norm(b) > 0
+
+
+@pytest.mark.gpu
+def test_experts_w4_refuses_weights_that_would_lose_their_gradient(ops, cuda):
+    rng = np.random.default_rng(30)
+    x, s = ops.quant_act(torch.from_numpy(rng.standard_normal((3, 128)).astype(np.float32)).to(cuda))
+    w13 = ops.pack_w4(*ops.quantize_w4(torch.from_numpy(rng.standard_normal((2, 256, 128)).astype(np.float32)).to(cuda)))
+    w2 = ops.pack_w4(*ops.quantize_w4(torch.from_numpy(rng.standard_normal((2, 128, 128)).astype(np.float32)).to(cuda)))
+    logits = torch.from_numpy(rng.standard_normal((3, 2)).astype(np.float32)).to(cuda).requires_grad_()
+    weights, ids = ops.route_topk(logits, None, 1)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.experts_w4(x, s, w13, w2, ids, weights)
+    want = ops.experts_w4(x, s, w13, w2, ids, weights.detach())
+    with torch.no_grad():
+        assert torch.equal(ops.experts_w4(x, s, w13, w2, *reversed(ops.route_topk(logits, None, 1))), want)
