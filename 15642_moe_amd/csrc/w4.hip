@@ -660,10 +660,12 @@ constexpr int ONLY_BIT = (int)0x80000000u, TOKEN_MASK = 0x7FFFFFFF;
 __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int inc = v;
+  if (__any(v)) {  // most waves' experts are none
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(inc, d);
-    if (lane >= d) inc += o;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
+    }
   }
   __syncthreads();
   if (lane == 63) s_wave[wave] = inc;
@@ -683,7 +685,8 @@ __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
 // with the shortest sum over GEMM1 (n1 weight blocks, k1 K-blocks) and GEMM2 is taken.
 struct TilePlan {
   int bm;  // a fixed size, or 0: chosen
-  int n1, k1, n2, k2, cus;
+  int n1, k1, n2, k2;
+  float per_cu;  // 1 / the workgroups that run at once
 };
 
 // Offsets and the tile list from expert `threadIdx.x`'s count: an expert's
@@ -700,26 +703,36 @@ __device__ __forceinline__ void publish_tiles(int cnt, int e_local, const TilePl
     __shared__ int s_sum[SIZES];
     if (e < SIZES) s_sum[e] = 0;
     __syncthreads();
+    if (__any(cnt)) {
 #pragma unroll
-    for (int i = 0; i < SIZES; ++i) {
-      const int m = (i + 2) * TILE_COLS;
-      int n = (cnt + m - 1) / m;
+      for (int i = 0; i < SIZES; ++i) {
+        const int m = (i + 2) * TILE_COLS;
+        int n = (cnt + m - 1) / m;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-      if ((e & 63) == 0 && n > 0) atomicAdd(&s_sum[i], n);
-    }
-    __syncthreads();
-    float least = 0.0f;
-    for (int i = SIZES - 1; i >= 0; --i) {
-      const int n = max(s_sum[i], 1);
-      const float item = (float)total / (float)(TILE_COLS * n) + 1.2f;
-      const float cost = item * ((float)((n * plan.n1 + plan.cus - 1) / plan.cus * plan.k1) +
-                                 (float)((n * plan.n2 + plan.cus - 1) / plan.cus * plan.k2));
-      if (i == SIZES - 1 || cost < least) {
-        least = cost;
-        bm = (i + 2) * TILE_COLS;
+        for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+        if ((e & 63) == 0) atomicAdd(&s_sum[i], n);
       }
     }
+    __syncthreads();
+    // Every lane the cost of size lane % SIZES, then all of them the least's (in equal
+    // cases the largest) size.
+    const int mine = e & (SIZES - 1);
+    const float n = (float)max(s_sum[mine], 1);
+    auto rounds = [&](int blocks) { return ceilf(n * (float)blocks * plan.per_cu - 1e-4f); };
+    const float item = (float)total * __builtin_amdgcn_rcpf(TILE_COLS * n) + 1.2f;
+    const float cost = item * (rounds(plan.n1) * (float)plan.k1 + rounds(plan.n2) * (float)plan.k2);
+    float least = cost;
+    int best = mine;
+#pragma unroll
+    for (int d = 1; d < SIZES; d <<= 1) {
+      const float o = __shfl_xor(least, d);
+      const int ob = __shfl_xor(best, d);
+      if (o < least || (o == least && ob > best)) {
+        least = o;
+        best = ob;
+      }
+    }
+    bm = (best + 2) * TILE_COLS;
   }
   const int tp = block_scan((cnt + bm - 1) / bm, s_wave, tiles);
   if (e < e_local) {
@@ -830,6 +843,13 @@ sort_place_kernel(const int32_t* __restrict__ ids, const float* __restrict__ wei
   place_picks(ids, weights, p0, min(picks, p0 + chunk), k, e_local, offset, s_pos, r);
 }
 
+// A route tile's entry, the same for all lanes: the weights' addresses stay in scalar
+// registers.
+__device__ __forceinline__ int4 uniform(const int4& t) {
+  return make_int4(__builtin_amdgcn_readfirstlane(t.x), __builtin_amdgcn_readfirstlane(t.y),
+                   __builtin_amdgcn_readfirstlane(t.z), __builtin_amdgcn_readfirstlane(t.w));
+}
+
 __device__ __forceinline__ float4 swiglu(const v4f& gate, const v4f& up) {
   auto one = [&](int i) { return up[i] / (1.0f + __expf(-up[i])) * gate[i]; };
   return make_float4(one(0), one(1), one(2), one(3));
@@ -858,7 +878,7 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
   const int KC = w4_chunks(a.H), KB = a.H / BLK, tiles = 2 * a.I / 16;
   for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
     if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
-    const int4 tile = r.tiles[i];
+    const int4 tile = uniform(r.tiles[i]);
     by_frags<MAXFR>(tile.z, [&](auto frc) __attribute__((always_inline)) {
       constexpr int FR = decltype(frc)::value;
       Stream<2 * NP, FR> st;
@@ -910,7 +930,7 @@ experts_gemm2_kernel(ExpertsW4 a, Routes r, const uint8_t* __restrict__ Cq,
   const int KC = w4_chunks(a.I), KB = a.I / BLK, tiles = a.H / 16;
   for (int i = blockIdx.x / slices; i < n_tiles; i += gridDim.x / slices) {
     if (i >= (int)(gridDim.x / slices)) __syncthreads();  // the waves have read the last tile's parts
-    const int4 tile = r.tiles[i];
+    const int4 tile = uniform(r.tiles[i]);
     by_frags<MAXFR>(tile.z, [&](auto frc) __attribute__((always_inline)) {
       constexpr int FR = decltype(frc)::value;
       Stream<NT, FR> st;
@@ -1105,10 +1125,10 @@ __device__ __forceinline__ void by_rows(int rows, F&& f) {
 
 // The tile and weight block of an item: experts in turn, an expert's items banded.
 __device__ __forceinline__ int4 expert_item(const Routes& r, int item, int nblk, int& nb) {
-  const int i = item / nblk, first = r.tiles[i].w;
+  const int i = item / nblk, first = __builtin_amdgcn_readfirstlane(r.tiles[i].w);
   int tile;
-  banded(item - first * nblk, nblk, r.tile_count[i], nb, tile);
-  return r.tiles[first + tile];
+  banded(item - first * nblk, nblk, __builtin_amdgcn_readfirstlane(r.tile_count[i]), nb, tile);
+  return uniform(r.tiles[first + tile]);
 }
 
 // GEMM1, SwiGLU and the FP8 requantisation of (route tile, 128 columns of the
@@ -1394,7 +1414,8 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   }
   const bool tile = experts_in_tiles(a);
   const int fr = a.T <= 16 ? 1 : 2;
-  const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK, device_cus() * (2 / TILE_CW)};
+  const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK,
+                         1.0f / (float)(device_cus() * (2 / TILE_CW))};
   if (picks <= SORT_SMALL) {
     sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
   } else {

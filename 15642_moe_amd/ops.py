@@ -245,16 +245,32 @@ def moe_forward(hidden, hidden_scale, W13_packed, W13_scale, W2_packed, W2_scale
 
 
 # --------------------------------------------------------------------------- general router
-# A call of these operators may take the GPU 3 us, so the host's share counts: with one C call on plain integers, the
-# device switched only where another one is current, and the stream read as a raw handle, route_topk takes the
-# host 9 us at T = 1 where wrapped pointers, the device and stream objects took 14.
+# A call of these operators may take the GPU 3 us, so the host's share counts: one C call on plain integers, devices
+# compared by their numbers, the device switched only where another one is current, and the stream read as a raw handle.
+# route_topk took the host 14 us at T = 1 with wrapped pointers, device and stream objects.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice  # a tensor on a device is there: the runtime is up
+_F32, _BF16, _F16, _I32, _U8, _E4M3 = (torch.float32, torch.bfloat16, torch.float16, torch.int32, torch.uint8,
+                                       torch.float8_e4m3fn)
 
 
-def _call(what: str, fn, dev: torch.device, *args) -> None:
-    """fn(*args, stream) with `dev` current, on its current stream; RuntimeError for a non-zero status."""
-    i = dev.index
-    if i == torch.cuda.current_device():
+def _index(name: str, t: torch.Tensor) -> int:
+    """The number of the HIP device that t is on."""
+    i = t.get_device()
+    if i < 0:
+        _require_device(name, t)
+    return i
+
+
+def _on(name: str, t: torch.Tensor, like: torch.Tensor, i: int) -> None:
+    """t is on the device of `like`, whose number is i."""
+    if t.get_device() != i:
+        _require_device(name, t, like.device)
+
+
+def _call(what: str, fn, i: int, *args) -> None:
+    """fn(*args, stream) with device i current, on its current stream; RuntimeError for a non-zero status."""
+    if i == _current_device():
         rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(i):
@@ -268,13 +284,14 @@ def _empty(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=dev)
 
 
-_DTYPES = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}
+_DTYPES = {_F32: capi.DTYPE_F32, _BF16: capi.DTYPE_BF16, _F16: capi.DTYPE_F16}
 
 
 def _rows(name: str, x: torch.Tensor) -> tuple:
-    """Checks a [T, n] float input and returns T, n and its row stride in elements."""
-    _require_device(name, x)
-    if x.dtype not in _DTYPES:
+    """Checks a [T, n] float input and returns T, n, its row stride in elements, its type and its device's number."""
+    i = _index(name, x)
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
     if x.dim() != 2:
         raise RuntimeError(f"{name} must be two-dimensional")
@@ -282,32 +299,33 @@ def _rows(name: str, x: torch.Tensor) -> tuple:
     stride, step = x.stride()
     if step != 1 and n != 1:
         raise RuntimeError(f"{name} must be contiguous along its last dimension")
-    return T, n, stride if T > 1 else n
+    return T, n, stride if T > 1 else n, dtype, i
 
 
 def _check_router(logits, top_k, scoring):
-    T, E, stride = _rows("logits", logits)
-    if scoring not in capi.SCORING:
+    T, E, stride, dtype, i = _rows("logits", logits)
+    score = capi.SCORING.get(scoring)
+    if score is None:
         raise RuntimeError(f"scoring must be one of {sorted(capi.SCORING)}, got {scoring!r}")
     if not 1 <= E <= capi.MAX_EXPERTS:
         raise RuntimeError(f"logits must have 1 to {capi.MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(capi.MAX_TOP_K, E):
         raise RuntimeError(f"top_k must be in [1, {min(capi.MAX_TOP_K, E)}], got {top_k}")
-    return T, E, stride
+    return T, E, stride, dtype, i, score
 
 
 def _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale):
-    T, E, stride = _check_router(logits, top_k, scoring)
+    T, E, stride, dtype, i, score = _check_router(logits, top_k, scoring)
     dev = logits.device
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous():
+        if bias.dtype != _F32 or bias.shape != (E,) or not bias.is_contiguous():
             raise RuntimeError(f"bias must be float32 [{E}] contiguous")
-        _require_device("bias", bias, dev)
-    weights = _empty(T, top_k, torch.float32, dev)
-    ids = _empty(T, top_k, torch.int32, dev)
-    _call("route_topk", capi.load().moe_route_topk, dev, logits.data_ptr(), _DTYPES[logits.dtype], stride,
-          None if bias is None else bias.data_ptr(), T, E, top_k, capi.SCORING[scoring], n_group, topk_group, group_top,
-          renormalize, scale, weights.data_ptr(), ids.data_ptr())
+        _on("bias", bias, logits, i)
+    weights = _empty(T, top_k, _F32, dev)
+    ids = _empty(T, top_k, _I32, dev)
+    _call("route_topk", capi.load().moe_route_topk, i, logits.data_ptr(), dtype, stride,
+          None if bias is None else bias.data_ptr(), T, E, top_k, score, n_group, topk_group, group_top, renormalize,
+          scale, weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -315,19 +333,19 @@ def route_topk_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: t
                         renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
     """The gradient of route_topk's logits [T, n_experts], in their type, from that of its weights (f32 [T, top_k])
     and its picks.  Picks outside [0, n_experts) (an unfilled slot's -1) take no part."""
-    _check(ids.dim() == 2 and ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be int32 [T, top_k] contiguous")
-    top_k = int(ids.size(1))
-    T, E, stride = _check_router(logits, top_k, scoring)
-    dev = logits.device
-    _check(ids.size(0) == T, "ids must have a row per token")
-    _check(grad_weights.dtype == torch.float32 and grad_weights.shape == ids.shape and grad_weights.is_contiguous(),
-           "grad_weights must be float32 [T, top_k] contiguous")
-    _require_device("ids", ids, dev)
-    _require_device("grad_weights", grad_weights, dev)
-    out = _empty(T, E, logits.dtype, dev)
-    _call("route_topk_backward", capi.load().moe_route_topk_backward, dev, grad_weights.data_ptr(), logits.data_ptr(),
-          _DTYPES[logits.dtype], stride, ids.data_ptr(), T, E, top_k, capi.SCORING[scoring], renormalize, scale,
-          out.data_ptr())
+    if ids.dim() != 2 or ids.dtype != _I32 or not ids.is_contiguous():
+        raise RuntimeError("ids must be int32 [T, top_k] contiguous")
+    rows, top_k = ids.shape
+    T, E, stride, dtype, i, score = _check_router(logits, top_k, scoring)
+    if rows != T:
+        raise RuntimeError("ids must have a row per token")
+    if grad_weights.dtype != _F32 or grad_weights.shape != ids.shape or not grad_weights.is_contiguous():
+        raise RuntimeError("grad_weights must be float32 [T, top_k] contiguous")
+    _on("ids", ids, logits, i)
+    _on("grad_weights", grad_weights, logits, i)
+    out = _empty(T, E, logits.dtype, logits.device)
+    _call("route_topk_backward", capi.load().moe_route_topk_backward, i, grad_weights.data_ptr(), logits.data_ptr(), dtype,
+          stride, ids.data_ptr(), T, E, top_k, score, renormalize, scale, out.data_ptr())
     return out
 
 
@@ -385,13 +403,14 @@ def _check_size(T: int, K: int) -> None:
 def quant_act(x: torch.Tensor):
     """[T, K] float32, bfloat16 or float16 (K a multiple of 128) -> (e4m3 [T, K], scale f32 [K / 128, T]): the
     quantisation that router_quant does on its way, for the input of linear_w4 and experts_w4 or moe_forward."""
-    T, K, stride = _rows("x", x)
+    T, K, stride, dtype, i = _rows("x", x)
     _check_size(T, K)
-    _check(stride * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0, "x must have 16-byte aligned rows")
-    codes = _empty(T, K, torch.float8_e4m3fn, x.device)
-    scale = _empty(K // 128, T, torch.float32, x.device)
-    _call("quant_act", capi.load().moe_quant_act, x.device, x.data_ptr(), _DTYPES[x.dtype], stride, T, K,
-          codes.data_ptr(), scale.data_ptr())
+    at, dev = x.data_ptr(), x.device
+    if stride * x.element_size() % 16 or at % 16:
+        raise RuntimeError("x must have 16-byte aligned rows")
+    codes = _empty(T, K, _E4M3, dev)
+    scale = _empty(K // 128, T, _F32, dev)
+    _call("quant_act", capi.load().moe_quant_act, i, at, dtype, stride, T, K, codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -407,7 +426,7 @@ def quantize_w4(w: torch.Tensor):
     _check(0 < K <= capi.MAX_W4_DIM and K % 128 == 0, f"w must have a multiple of 128 columns, got {K}")
     codes = torch.empty((*w.shape[:-1], K // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((*w.shape[:-1], K // W4_GROUP), dtype=torch.uint8, device=w.device)
-    _call("quantize_w4", capi.load().moe_quantize_w4, w.device, w.data_ptr(), _DTYPES[w.dtype], w.numel() // W4_GROUP,
+    _call("quantize_w4", capi.load().moe_quantize_w4, w.get_device(), w.data_ptr(), _DTYPES[w.dtype], w.numel() // W4_GROUP,
           codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -438,56 +457,57 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None 
         _check(out.dtype == torch.uint8 and tuple(out.shape) == shape and out.is_contiguous(),
                f"pack_w4 out must be uint8 {list(shape)} contiguous")
         _require_device("pack_w4 out", out, codes.device)
-    _call("pack_w4", capi.load().moe_pack_w4, codes.device, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, N, K)
+    _call("pack_w4", capi.load().moe_pack_w4, codes.get_device(), codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, N, K)
     return out
 
 
 def unpack_w4(packed: torch.Tensor, N: int, K: int):
     """Inverse of pack_w4: (codes uint8 [.., N, K / 2], scales uint8 [.., N, K / 32])."""
+    _require_device("packed", packed)
     _check_packed("packed", packed, N, K, batched=packed.dim() == 4)
     lead = packed.shape[:-3]
     codes = torch.empty((*lead, N, K // 2), dtype=torch.uint8, device=packed.device)
     scales = torch.empty((*lead, N, K // W4_GROUP), dtype=torch.uint8, device=packed.device)
     n = int(packed.size(0)) if packed.dim() == 4 else 1
-    _call("unpack_w4", capi.load().moe_unpack_w4, packed.device, packed.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+    _call("unpack_w4", capi.load().moe_unpack_w4, packed.get_device(), packed.data_ptr(), codes.data_ptr(), scales.data_ptr(),
           n, N, K)
     return codes, scales
 
 
-def _check_packed(name, packed, N, K, batched, device=None):
-    _require_device(name, packed, device)
+def _check_packed(name, packed, N, K, batched):
     want = _w4_shape(N, K)
-    if packed.dtype != torch.uint8 or packed.dim() != 3 + batched or packed.shape[-3:] != want \
-            or not packed.is_contiguous():
+    if packed.dtype != _U8 or packed.dim() != 3 + batched or packed.shape[-3:] != want or not packed.is_contiguous():
         lead = "[e_local, " if batched else "["
         raise RuntimeError(f"{name} must be a pack_w4 result uint8 {lead}{want[0]}, {want[1]}, {want[2]}] contiguous, "
                            f"got {packed.dtype} {list(packed.shape)}")
 
 
 def _check_act(x, x_scale):
-    _require_device("x", x)
-    dev = x.device
-    _require_device("x_scale", x_scale, dev)
-    _check(x.dtype == torch.float8_e4m3fn and x.dim() == 2 and x.is_contiguous(), "x must be e4m3 [T, K] contiguous")
+    i = _index("x", x)
+    _on("x_scale", x_scale, x, i)
+    if x.dtype != _E4M3 or x.dim() != 2 or not x.is_contiguous():
+        raise RuntimeError("x must be e4m3 [T, K] contiguous")
     T, K = x.shape
     _check_size(T, K)
-    if x_scale.dtype != torch.float32 or x_scale.shape != (K // 128, T) or not x_scale.is_contiguous():
+    if x_scale.dtype != _F32 or x_scale.shape != (K // 128, T) or not x_scale.is_contiguous():
         raise RuntimeError(f"x_scale must be float32 [{K // 128}, {T}] contiguous")
-    return T, K, dev
+    return T, K, i
 
 
 def linear_w4(x: torch.Tensor, x_scale: torch.Tensor, packed: torch.Tensor, n_out: int | None = None) -> torch.Tensor:
     """bf16 [T, N] = x W^T for a dense layer in 4 bits: x and x_scale from quant_act (or router_quant), `packed` from
     pack_w4.  `n_out` is N where it is not a multiple of 16."""
-    T, K, dev = _check_act(x, x_scale)
-    _check(packed.dim() == 3, "packed must be a pack_w4 result [row tiles, chunks, 4352]")
-    tiles = int(packed.size(0))
+    T, K, i = _check_act(x, x_scale)
+    if packed.dim() != 3:
+        raise RuntimeError("packed must be a pack_w4 result [row tiles, chunks, 4352]")
+    tiles = packed.size(0)
     N = 16 * tiles if n_out is None else int(n_out)
     if not 16 * (tiles - 1) < N <= 16 * tiles:
         raise RuntimeError(f"n_out must be in [{16 * tiles - 15}, {16 * tiles}] for {tiles} packed row tiles, got {N}")
-    _check_packed("packed", packed, N, K, False, dev)
-    out = _empty(T, N, torch.bfloat16, dev)
-    _call("linear_w4", capi.load().moe_linear_w4, dev, x.data_ptr(), x_scale.data_ptr(), packed.data_ptr(), T, N, K,
+    _on("packed", packed, x, i)
+    _check_packed("packed", packed, N, K, False)
+    out = _empty(T, N, _BF16, x.device)
+    _call("linear_w4", capi.load().moe_linear_w4, i, x.data_ptr(), x_scale.data_ptr(), packed.data_ptr(), T, N, K,
           out.data_ptr())
     return out
 
@@ -501,27 +521,31 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     int32 [T, top_k] and weights f32 [T, top_k] as route_topk gives them.  Picks outside [local_offset, local_offset +
     e_local) are another rank's, or none, and add nothing; a token without local picks gets zeros.  hidden and inter
     are multiples of 128.  For serving: it has no gradient, and refuses weights that would lose theirs."""
-    T, K, dev = _check_act(x, x_scale)
-    _check(w13.dim() == 4 and w2.dim() == 4, "w13 and w2 must be pack_w4 results [e_local, row tiles, chunks, 4352]")
-    E, inter = int(w13.size(0)), 8 * int(w13.size(1))
+    T, K, i = _check_act(x, x_scale)
+    if w13.dim() != 4 or w2.dim() != 4:
+        raise RuntimeError("w13 and w2 must be pack_w4 results [e_local, row tiles, chunks, 4352]")
+    E, inter = w13.size(0), 8 * w13.size(1)
     _check(inter % 128 == 0, "w13 must have 2 * inter rows, inter a multiple of 128")
-    _check_packed("w13", w13, 2 * inter, K, True, dev)
-    _check_packed("w2", w2, K, inter, True, dev)
-    _check(w2.size(0) == E, "w13 and w2 must have the same experts")
-    _check(ids.dim() == 2 and ids.dtype == torch.int32 and ids.size(0) == T and ids.is_contiguous(),
-           "ids must be int32 [T, top_k] contiguous")
-    _check(weights.dtype == torch.float32 and weights.shape == ids.shape and weights.is_contiguous(),
-           "weights must be float32 [T, top_k] contiguous")
-    _require_device("ids", ids, dev)
-    _require_device("weights", weights, dev)
-    _check(not (weights.requires_grad and torch.is_grad_enabled()),
-           "experts_w4 has no gradient: call it under torch.no_grad(), or with weights.detach()")
-    k = int(ids.size(1))
+    _on("w13", w13, x, i)
+    _on("w2", w2, x, i)
+    _check_packed("w13", w13, 2 * inter, K, True)
+    _check_packed("w2", w2, K, inter, True)
+    if w2.size(0) != E:
+        raise RuntimeError("w13 and w2 must have the same experts")
+    if ids.dim() != 2 or ids.dtype != _I32 or ids.size(0) != T or not ids.is_contiguous():
+        raise RuntimeError("ids must be int32 [T, top_k] contiguous")
+    if weights.dtype != _F32 or weights.shape != ids.shape or not weights.is_contiguous():
+        raise RuntimeError("weights must be float32 [T, top_k] contiguous")
+    _on("ids", ids, x, i)
+    _on("weights", weights, x, i)
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("experts_w4 has no gradient: call it under torch.no_grad(), or with weights.detach()")
+    k, dev = ids.size(1), x.device
     lib = capi.load()
-    ws_bytes = int(lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k))
-    out = _empty(T, K, torch.bfloat16, dev)
-    ws = _empty(1, max(ws_bytes, 1), torch.uint8, dev)
-    _call("experts_w4", lib.moe_experts_w4, dev, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+    ws_bytes = lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k)
+    out = _empty(T, K, _BF16, dev)
+    ws = _empty(1, max(ws_bytes, 1), _U8, dev)
+    _call("experts_w4", lib.moe_experts_w4, i, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
           ids.data_ptr(), weights.data_ptr(), T, K, inter, E, k, local_offset, ws.data_ptr(), ws_bytes, out.data_ptr())
     return out
 
