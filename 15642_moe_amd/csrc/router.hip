@@ -187,7 +187,8 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Token t by one wave; lane l holds experts EPL*l .. +EPL.
+// Token t by one wave; lane l holds experts EPL*l .. +EPL.  Bound by the latency of k
+// rounds of a wave-wide maximum: 256 experts in 8 groups, top 8, T = 1 in 4.3 us.
 template <int EPL, int DT, bool SOFTMAX>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int t, RouteLds<EPL>& s) {
   const int lane = threadIdx.x & 63;

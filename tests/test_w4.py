@@ -636,3 +636,20 @@ def test_experts_w4_refuses_weights_that_would_lose_their_gradient(ops, cuda):
     want = ops.experts_w4(x, s, w13, w2, ids, weights.detach())
     with torch.no_grad():
         assert torch.equal(ops.experts_w4(x, s, w13, w2, *reversed(ops.route_topk(logits, None, 1))), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantize_w4_every_value(ops, cuda, dtype):
+    """Every finite value of a 16-bit type, in groups whose largest element lies up to three binades above it."""
+    every = torch.arange(1 << 16).to(torch.int32).to(torch.int16).view(dtype)
+    every = every[every.isfinite()]
+    for up in (0, 1, 2, 3):
+        top = torch.minimum(every.float().abs() * 2.0**up * 1.5, torch.tensor(torch.finfo(dtype).max))
+        w = torch.zeros(every.numel(), 32)
+        w[:, ::4], w[:, 1] = every.float()[:, None], top
+        w = w.to(dtype).view(-1, 128)
+        codes, scales = ops.quantize_w4(w.to(cuda))
+        want, want_s = oracle.quantize(w.float().numpy())
+        assert np.array_equal(scales.cpu().numpy(), want_s)
+        assert np.array_equal(codes.cpu().numpy(), want)
