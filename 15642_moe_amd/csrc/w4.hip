@@ -396,7 +396,7 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 // rows with up to 64 activation rows, two workgroups a CU: a wave takes 4 weight tiles
 // and all the rows.  The weights go from global memory to the registers of the wave
 // that owns their rows, three K-blocks ahead; the activations, which every wave
-// needs, go through LDS, a step of two K-blocks ahead.  Per K-block a wave reads 2 KB
+// needs, go through LDS, a step of two or four K-blocks ahead.  Per K-block a wave reads 2 KB
 // of LDS for each four MFMAs (128 clocks of its SIMD): half of the LDS bandwidth with
 // two waves a SIMD.  What bounds it: the MFMAs take 37% of the clocks and the scales'
 // multiply-adds (four a product) and addresses another 40%, beside each other only where
@@ -409,10 +409,14 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 // ---------------------------------------------------------------------------
 constexpr int TILE_ROWS = 256, TILE_CW = 1, TILE_THREADS = 256 * TILE_CW, TILE_MAX_NC = 5;
 constexpr int TILE_COLS = 16 * TILE_CW, TILE_MAX_M = TILE_COLS * TILE_MAX_NC;  // activation rows
-constexpr int STEP_BLOCKS = 2;  // K-blocks of activations that are staged at once
+// K-blocks of activations that are staged at once, between two barriers: four where they are
+// few (N = 4096, K = 7168: T = 128 16.5 us with two, 14.9 with four; T = 256 19.7 and 16.7).
+constexpr int step_blocks(int nc) { return nc <= 2 ? 4 : 2; }
+constexpr int STEP_ROWS = 2 * TILE_MAX_M;  // rows times K-blocks of a step at most
+static_assert(2 * TILE_COLS * step_blocks(2) <= STEP_ROWS, "a step of the small tiles");
 struct TileLds {
-  uint8_t x[2][STEP_BLOCKS * TILE_MAX_M * BLK];  // [K-block][row][128]
-  float xs[2][STEP_BLOCKS * TILE_MAX_M];
+  uint8_t x[2][STEP_ROWS * BLK];  // [K-block][row][128]
+  float xs[2][STEP_ROWS];
   size_t row[TILE_MAX_M];  // byte offset of each activation row
   union {
     float amax[4][TILE_MAX_M];  // GEMM1
@@ -432,7 +436,7 @@ template <int NC, class RowOf>
 __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&w)[4], int K, const uint8_t* x,
                                              const float* xs, size_t xs_row, size_t xs_block, RowOf&& row_of,
                                              v4f (&acc)[4][NC]) {
-  constexpr int M = TILE_COLS * NC, NR = W4_CHUNK_BLOCKS, NS = STEP_BLOCKS;
+  constexpr int M = TILE_COLS * NC, NR = W4_CHUNK_BLOCKS, NS = step_blocks(NC);
   constexpr int PIECES = NS * 8, PER = M * PIECES / TILE_THREADS;  // 16-byte pieces of a row's step, and per thread
   const int tid = threadIdx.x, lane = tid & 63, KB = K / BLK, last = (KB - 1) / NR;
   const int cw = __builtin_amdgcn_readfirstlane(tid >> 8);
@@ -442,14 +446,21 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   const int piece = tid % PIECES, row0 = tid / PIECES;
   const float* scale = xs + (size_t)row_of(tid % M) * xs_row + (size_t)(tid / M) * xs_block;
   if (tid < M) s.row[tid] = (size_t)row_of(tid) * K;
+  constexpr bool IN_REGS = NC <= 2;  // the rows' addresses, else read again for each step
+  const uint8_t* rows[IN_REGS ? PER : 1];
+  auto row_at = [&](int i) __attribute__((always_inline)) {
+    return x + s.row[row0 + i * (TILE_THREADS / PIECES)] + (piece & 7) * 16;
+  };
   u32x4 st[PER];
   float ss = 0.0f;
   // Piece i of a step: its load (past the end of K: anything), and its write to LDS
   // (zeros there, which the padded weights need: a NaN code times zero is NaN).
   auto fetch = [&](int step, int i) __attribute__((always_inline)) {
     const int kb = step * NS + (piece >> 3);
-    st[i] = *reinterpret_cast<const u32x4*>(x + s.row[row0 + i * (TILE_THREADS / PIECES)] +
-                                            (size_t)(kb < KB ? kb : 0) * BLK + (piece & 7) * 16);
+    const uint8_t* row;
+    if constexpr (IN_REGS) row = rows[i];
+    else row = row_at(i);
+    st[i] = *reinterpret_cast<const u32x4*>(row + (size_t)(kb < KB ? kb : 0) * BLK);
   };
   auto stage = [&](int step, int i) __attribute__((always_inline)) {
     if (step * NS + (piece >> 3) >= KB) st[i] = u32x4{0, 0, 0, 0};
@@ -487,6 +498,10 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   load_a(0, std::integral_constant<int, 2>{});
   fetch_scale(0);
   __syncthreads();
+  if constexpr (IN_REGS) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rows[i] = row_at(i);
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) fetch(0, i);
 #pragma unroll
@@ -504,8 +519,8 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
     static_for<NR / NS>([&](auto hc) __attribute__((always_inline)) {
       constexpr int h = decltype(hc)::value;
       const int step = chunk * (NR / NS) + h;
-      const uint8_t* xb = s.x[h & 1];
-      const float* xsb = s.xs[h & 1];
+      const uint8_t* xb = s.x[step & 1];
+      const float* xsb = s.xs[step & 1];
       // Fragment j of the step: K-block j / NC, rows 16 (j % NC) ..; its LDS reads run one
       // fragment ahead of its MFMAs.  Between the first half of the fragments the next
       // step's activations go to LDS (past the last: the buffer takes zeros), between
@@ -1144,7 +1159,8 @@ __device__ __forceinline__ int4 expert_item(const Routes& r, int item, int nblk,
 // GEMM1, SwiGLU and the FP8 requantisation of (route tile, 128 columns of the
 // intermediate): wave rw's weight tiles are 32 gate and the same 32 up rows.  7168, 2048,
 // 32 of 256 experts, T = 4001: 164 us, 1.4 PFLOP/s; GEMM2 106 us, 1.1 with its fp32 rows.
-// T = 64 on three experts: 31 us, the K loop's own time on 48 workgroups.
+// T = 64 on six experts: 28 us for 94 MB, which 96 workgroups' loads bound (a CU streams
+// 35 to 65 GB/s, however far ahead it loads).
 __global__ void __launch_bounds__(TILE_THREADS, 2)
 experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__ Cq, float* __restrict__ Cs) {
   __shared__ __align__(16) TileLds s;
