@@ -1353,10 +1353,12 @@ hipError_t launch_quant_act(const void* x, int dtype, size_t row_stride, int T, 
 
 // Whether a dense product runs in tiles.  A tile launch of few items takes its K loop's
 // time, a stream's time goes with the outputs; us, tiles / streams:
-//   N=4096 K=7168  T=64 24.0 / 12.6, 128 23.9 / 20.7, 192 23.6 / 30.4
-//   N=7168 K=2048  T=33 7.6 / 7.4, 48 7.6 / 8.1, 128 7.8 / 12.8
-//   N=1024 K=1024  T=256 5.2 / 4.6;  N=512 K=7168  T=256 16.7 / 11.8
-static bool linear_in_tiles(int T, int N, int K) { return (size_t)T * N > 300000 + 30 * (size_t)K; }
+//   N=4096 K=7168  T=64 20.6 / 12.6, 96 20.3 / 20.1, 128 20.1 / 20.6, 192 20.4 / 30.2
+//   N=2048 K=4096  T=128 9.8 / 8.3, 192 10.2 / 12.6
+//   N=7168 K=2048  T=32 7.0 / 6.4, 33 7.0 / 7.4, 128 7.3 / 12.9
+//   N=2000 K=512   T=64 4.2 / 4.5, 128 4.2 / 4.9
+//   N=1024 K=1024  T=256 4.9 / 4.6;  N=512 K=7168  T=256 14.4 / 11.7
+static bool linear_in_tiles(int T, int N, int K) { return (size_t)T * N > 150000 + 45 * (size_t)K; }
 
 // Fragments per wave of a tile launch: the fewest whole rounds of workgroups over
 // the CUs, each as long as its fragments and a constant share (weights, barriers).
@@ -1408,10 +1410,10 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
 
 // Whether the experts' products run in tiles: from 49 tokens on where a tile per
 // expert fills the CUs, else from 385 on.  Whole call, us, tiles / streams:
-//   7168, 2048, 32 of 256, top 8   even T=32 112 / 111, 64 133 / 142, 128 146 / 160, 512
-//     170 / 252; uneven T=32 53 / 50, 64 57 / 57, 128 61 / 77, 512 93 / 209
-//   2048, 768, 128 of 128, top 8   even T=32 75 / 74, 64 84 / 85, 512 111 / 178
-//   1024, 512, 16 of 64, top 4 (64 items)   even T=64 21 / 18, 256 25 / 22, 512 26 / 26
+//   7168, 2048, 32 of 256, top 8   even T=32 108 / 111, 64 126 / 137, 128 143 / 160, 512
+//     167 / 249; uneven T=32 50 / 45, 64 54 / 58, 128 58 / 79, 512 87 / 186
+//   2048, 768, 128 of 128, top 8   even T=32 69 / 74, 64 78 / 84, 512 109 / 177
+//   1024, 512, 16 of 64, top 4 (64 items)   even T=64 19 / 18, 256 23 / 22, 512 25 / 26
 static bool experts_in_tiles(const ExpertsW4& a) {
   return a.T > ((long long)a.e_local * (a.I / BLK) >= device_cus() ? 48 : 384);
 }

@@ -653,3 +653,10 @@ def test_quantize_w4_every_value(ops, cuda, dtype):
         want, want_s = oracle.quantize(w.float().numpy())
         assert np.array_equal(scales.cpu().numpy(), want_s)
         assert np.array_equal(codes.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K", [(86, 2000, 512), (87, 2000, 512), (33, 7168, 2048), (35, 7168, 1920), (190, 1030, 896)])
+def test_linear_w4_streams_and_tiles(ops, cuda, T, N, K):
+    """Either side of the sizes from which the product runs in tiles."""
+    _check_linear(ops, cuda, np.random.default_rng(T + N + K), T, N, K)
