@@ -666,7 +666,7 @@ struct Routes {
   int32_t* pick_route;   // [T k], -1 for picks of other experts
   int32_t* chunk_counts; // [chunks][e_local]
 };
-// One workgroup sorts up to SORT_SMALL picks (its atomics on a few experts' counters take
+// One launch sorts up to SORT_SMALL picks (its atomics on a few experts' counters take
 // 3 ns a pick); more are cut into at most SORT_MAX_CHUNKS chunks of at least
 // SORT_THREADS.
 constexpr int SORT_THREADS = 1024, SORT_SMALL = 2048, SORT_MAX_CHUNKS = 64;
@@ -813,7 +813,8 @@ __device__ __forceinline__ void count_picks(const int32_t* __restrict__ ids, int
   }
 }
 
-// All picks by one workgroup.
+// All picks, counted by both of two workgroups: the first publishes the offsets and the
+// tiles, the second places the picks (512 of them: 6.7 us by one after the other, 4.7 so).
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_small_kernel(const int32_t* __restrict__ ids, const float* __restrict__ weights, int picks, int k, int e_local, int offset, TilePlan plan, Routes r) {
   __shared__ int s_cnt[MAX_EXPERTS], s_off[MAX_EXPERTS], s_tp[MAX_EXPERTS], s_pos[MAX_EXPERTS], s_wave[16];
@@ -822,9 +823,14 @@ sort_small_kernel(const int32_t* __restrict__ ids, const float* __restrict__ wei
   __syncthreads();
   count_picks(ids, 0, picks, e_local, offset, s_pos);
   __syncthreads();
-  publish_tiles(tid < e_local ? s_pos[tid] : 0, e_local, plan, r, s_off, s_tp, s_cnt, s_wave);
-  __syncthreads();
-  s_pos[tid] = tid < e_local ? s_off[tid] : 0;
+  const int cnt = tid < e_local ? s_pos[tid] : 0;
+  if (blockIdx.x == 0) {
+    publish_tiles(cnt, e_local, plan, r, s_off, s_tp, s_cnt, s_wave);
+    return;
+  }
+  int all;
+  const int off = block_scan(cnt, s_wave, all);  // its barriers are behind everyone's reads
+  s_pos[tid] = off;
   __syncthreads();
   place_picks(ids, weights, 0, picks, k, e_local, offset, s_pos, r);
 }
@@ -1449,7 +1455,7 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK,
                          1.0f / (float)(device_cus() * (2 / TILE_CW))};
   if (picks <= SORT_SMALL) {
-    sort_small_kernel<<<1, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
+    sort_small_kernel<<<2, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
   } else {
     const int chunk = sort_chunk(picks), chunks = (picks + chunk - 1) / chunk;
     sort_count_kernel<<<chunks, SORT_THREADS, 0, stream>>>(a.ids, picks, chunk, a.e_local, a.offset, r);
