@@ -356,3 +356,50 @@ def test_route_topk_backward_many_tokens(ops, cuda, E, k, dtype):
             _check_grad(got[rows], g[rows], x[rows], ids[rows], "softmax", renormalize, 2.5)
             _check_grad(one, g[rows], x[rows], ids[rows], "softmax", renormalize, 2.5)
             assert torch.equal(got, ops.route_topk_backward(g, x, ids, "softmax", renormalize, 2.5))
+
+
+@pytest.mark.gpu
+def test_route_topk_far_rows(ops, cuda):
+    """The largest batch: elements past 2^31, and past 2^32 bytes."""
+    T, E = 1 << 24, 256
+    x = torch.empty(T, E, dtype=torch.bfloat16, device=cuda)
+    x[: 1 << 20] = torch.randn(1 << 20, E, device=cuda).to(torch.bfloat16)
+    for i in range(1, 16):
+        x[i << 20 : (i + 1) << 20] = x[: 1 << 20].roll(i, 0)
+    w, ids = ops.route_topk(x, None, 8, "softmax", 8, 4)
+    g = torch.randn(1 << 20, 8, device=cuda).repeat(16, 1)
+    dx = ops.route_topk_backward(g, x, ids, "softmax")
+    for lo in (0, T // 2 - 4500, T - 9000):
+        rows = slice(lo, lo + 9000)  # 8192 and more: the same layout, and order of sums, as the whole batch
+        want = ops.route_topk(x[rows], None, 8, "softmax", 8, 4)
+        assert torch.equal(w[rows], want[0]) and torch.equal(ids[rows], want[1])
+        assert torch.equal(dx[rows], ops.route_topk_backward(g[rows], x[rows], ids[rows], "softmax"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_route_topk_captured_training_step(ops, cuda, scoring):
+    """Forward and backward in a graph, replayed over new logits with eager work between."""
+    x = _logits(300, 160, 61, torch.float32, "plain").to(cuda).requires_grad_()
+    g = torch.randn(300, 6, generator=torch.Generator().manual_seed(8)).to(cuda)
+
+    def step():
+        w, ids = ops.route_topk(x, None, 6, scoring, 8, 3)
+        return w.detach(), ids, torch.autograd.grad(w, x, g)[0]  # nothing of the autograd graph stays
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(_logits(300, 160, 70 + seed, torch.float32, "plain"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)

@@ -660,3 +660,77 @@ def test_quantize_w4_every_value(ops, cuda, dtype):
 def test_linear_w4_streams_and_tiles(ops, cuda, T, N, K):
     """Either side of the sizes from which the product runs in tiles."""
     _check_linear(ops, cuda, np.random.default_rng(T + N + K), T, N, K)
+
+
+@pytest.mark.gpu
+def test_experts_w4_far_weights(ops, cuda):
+    """Experts past 2^32 bytes of packed weights: each form on the last ones, against a view of theirs alone."""
+    E, hidden, inter = 300, 7168, 2048
+    w13 = torch.full((E, 2 * inter // 16, hidden // 512, 4352), 0x71, dtype=torch.uint8, device=cuda)
+    w2 = torch.full((E, hidden // 16, inter // 512, 4352), 0x71, dtype=torch.uint8, device=cuda)
+    assert w13.numel() > 1 << 32
+    w13[-2:, ..., :4096].random_(0, 256)
+    w2[-2:, ..., :4096].random_(0, 256)
+    rng = np.random.default_rng(31)
+    for T in (1, 40, 70):
+        xc, xs = _act(rng, T, hidden)
+        x, s = _dev(xc, cuda, F8), _dev(xs, cuda)
+        ids = _dev(rng.integers(E - 2, E, size=(T, 2)).astype(np.int32), cuda)
+        weights = _dev(rng.uniform(0.1, 1, (T, 2)).astype(np.float32), cuda)
+        got = ops.experts_w4(x, s, w13, w2, ids, weights)
+        # 32 experts, so that the same form is taken
+        want = ops.experts_w4(x, s, w13[-32:], w2[-32:], ids, weights, E - 32)
+        assert torch.equal(got, want) and got.count_nonzero() > 0
+
+
+@pytest.mark.gpu
+def test_linear_w4_far_rows(ops, cuda):
+    """Activations past 2^32 bytes and outputs past 2^31 elements."""
+    T, K, N = 200_000, 16_384, 11_008
+    x = torch.empty(T, K, dtype=torch.bfloat16, device=cuda)
+    x[:20_000] = torch.randn(20_000, K, device=cuda).to(torch.bfloat16)
+    for i in range(1, 10):
+        x[20_000 * i : 20_000 * (i + 1)] = x[:20_000].roll(i, 0)
+    codes, scale = ops.quant_act(x)
+    p = torch.full((N // 16, K // 512, 4352), 0x71, dtype=torch.uint8, device=cuda)
+    p[..., :4096].random_(0, 256)
+    y = ops.linear_w4(codes, scale, p)
+    for lo in (0, 97_000, T - 4096):
+        rows = slice(lo, lo + 4096)
+        c, s = ops.quant_act(x[rows])
+        assert torch.equal(c.view(torch.uint8), codes[rows].view(torch.uint8)) and torch.equal(s, scale[:, rows])
+        assert torch.equal(ops.linear_w4(c, s, p), y[rows])
+
+
+@pytest.mark.gpu
+def test_w4_two_graphs(ops, cuda):
+    """Two captured calls, replayed in turn and over each other on two streams: each has its own workspace."""
+    rng = np.random.default_rng(33)
+    w13 = ops.pack_w4(_dev(_codes(rng, 4, 1024, 256), cuda), torch.full((4, 1024, 16), 118, dtype=torch.uint8, device=cuda))
+    w2 = ops.pack_w4(_dev(_codes(rng, 4, 512, 256), cuda), torch.full((4, 512, 16), 118, dtype=torch.uint8, device=cuda))
+    runs, held = [], []
+    for T in (390, 400):
+        xc, xs = _act(rng, T, 512)
+        args = (_dev(xc, cuda, F8), _dev(xs, cuda), w13, w2, _dev(rng.integers(0, 4, (T, 3)).astype(np.int32), cuda),
+                _dev(rng.uniform(0.1, 1, (T, 3)).astype(np.float32), cuda))
+        want = ops.experts_w4(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.experts_w4(*args)
+        runs.append((graph, out, want, torch.cuda.Stream()))
+        held.append(args)  # a replay reads them
+    for _ in range(3):
+        for graph, out, want, _ in runs:
+            out.zero_()
+            graph.replay()
+        for graph, out, want, _ in runs:
+            assert torch.equal(out, want)
+        torch.cuda.synchronize()
+        for graph, _, _, stream in runs:
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in runs:
+            assert torch.equal(out, want)
