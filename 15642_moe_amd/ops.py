@@ -10,6 +10,7 @@ device.  There is no CPU path: CPU tensors raise RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -512,6 +513,11 @@ def linear_w4(x: torch.Tensor, x_scale: torch.Tensor, packed: torch.Tensor, n_ou
     return out
 
 
+@functools.lru_cache(256)  # of sizes alone: 0.1 us, where the call takes 0.5
+def _experts_w4_workspace(T: int, hidden: int, inter: int, e_local: int, top_k: int) -> int:
+    return capi.load().moe_experts_w4_workspace_bytes(T, hidden, inter, e_local, top_k)
+
+
 def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, ids: torch.Tensor,
                weights: torch.Tensor, local_offset: int = 0) -> torch.Tensor:
     """bf16 [T, hidden]: the routed experts of moe_forward with 4-bit weights, on the picks of any router.
@@ -541,11 +547,10 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     if weights.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("experts_w4 has no gradient: call it under torch.no_grad(), or with weights.detach()")
     k, dev = ids.size(1), x.device
-    lib = capi.load()
-    ws_bytes = lib.moe_experts_w4_workspace_bytes(T, K, inter, E, k)
+    ws_bytes = _experts_w4_workspace(T, K, inter, E, k)
     out = _empty(T, K, _BF16, dev)
     ws = _empty(1, max(ws_bytes, 1), _U8, dev)
-    _call("experts_w4", lib.moe_experts_w4, i, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+    _call("experts_w4", capi.load().moe_experts_w4, i, x.data_ptr(), x_scale.data_ptr(), w13.data_ptr(), w2.data_ptr(),
           ids.data_ptr(), weights.data_ptr(), T, K, inter, E, k, local_offset, ws.data_ptr(), ws_bytes, out.data_ptr())
     return out
 
