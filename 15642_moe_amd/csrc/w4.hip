@@ -407,8 +407,8 @@ linear_w4_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
 // LDS rows are 128 bytes; the 16-byte piece q of row m lies at position q ^ (m & 7),
 // so that eight lanes with eight consecutive rows read eight different banks' groups.
 // ---------------------------------------------------------------------------
-constexpr int TILE_ROWS = 256, TILE_CW = 1, TILE_THREADS = 256 * TILE_CW, TILE_MAX_NC = 5;
-constexpr int TILE_COLS = 16 * TILE_CW, TILE_MAX_M = TILE_COLS * TILE_MAX_NC;  // activation rows
+constexpr int TILE_ROWS = 256, TILE_THREADS = 256, TILE_MAX_NC = 5, TILE_WGS = 2;  // workgroups a CU
+constexpr int TILE_COLS = 16, TILE_MAX_M = TILE_COLS * TILE_MAX_NC;                 // activation rows
 // K-blocks of activations that are staged at once, between two barriers: four where they are
 // few (N = 4096, K = 7168: T = 128 16.5 us with two, 14.9 with four; T = 256 19.7 and 16.7).
 constexpr int step_blocks(int nc) { return nc <= 2 ? 4 : 2; }
@@ -439,7 +439,6 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   constexpr int M = TILE_COLS * NC, NR = W4_CHUNK_BLOCKS, NS = step_blocks(NC);
   constexpr int PIECES = NS * 8, PER = M * PIECES / TILE_THREADS;  // 16-byte pieces of a row's step, and per thread
   const int tid = threadIdx.x, lane = tid & 63, KB = K / BLK, last = (KB - 1) / NR;
-  const int cw = __builtin_amdgcn_readfirstlane(tid >> 8);
   const v4f zero4 = {0.f, 0.f, 0.f, 0.f};
   // Thread tid fetches one piece of the step's K-blocks of rows tid / PIECES +
   // (TILE_THREADS / PIECES) i, and the scale of row tid % M, K-block tid / M.
@@ -511,7 +510,7 @@ __device__ __forceinline__ void tile_product(TileLds& s, const uint8_t* const (&
   for (int i = 0; i < PER; ++i) fetch(1, i);
   fetch_scale(1);
   __syncthreads();
-  const int i16 = cw * (16 * NC) + (lane & 15), g = lane >> 4;
+  const int i16 = lane & 15, g = lane >> 4;
 #pragma unroll 1
   for (int chunk = 0; chunk <= last; ++chunk) {
 #pragma unroll
@@ -591,12 +590,12 @@ void by_grids(size_t items, F&& f) {
 }
 
 template <int NC>
-__global__ void __launch_bounds__(TILE_THREADS, 2)
+__global__ void __launch_bounds__(TILE_THREADS, TILE_WGS)
 linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs, const uint8_t* __restrict__ packed,
                       int T, int N, int K, int base, uint16_t* __restrict__ out) {
   __shared__ __align__(16) TileLds s;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(K), tiles = w4_tiles(N), blocks = (tiles + 15) / 16;
   const int token_tiles = (T + TILE_COLS * NC - 1) / (TILE_COLS * NC);
   const int item = xcd_item(base, blocks * token_tiles);
@@ -615,36 +614,31 @@ linear_w4_tile_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x
   // activations' are, so that 32 lanes store 512 contiguous bytes (straight from the
   // registers, 8 bytes a lane, the stores took 8 of 37 us at T = 1501, N = 7168, K = 2048).
   uint8_t* tile = s.x[0];
-  constexpr int HALF = 16 * NC;  // rows at a time, a wave column's: 512 bytes each
-  static_assert(HALF * 512 <= (int)sizeof(s.x), "a wave column's rows");
+  constexpr int M = 16 * NC;
+  static_assert(M * 512 <= (int)sizeof(s.x), "the tile in bf16");
   const int n0 = nb * TILE_ROWS;
-  for (int half = 0; half < TILE_CW; ++half) {
-    if (half > 0) __syncthreads();
-    if (cw == half) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int m = c * 16 + (lane & 15);
+  for (int c = 0; c < NC; ++c) {
+    const int m = c * 16 + (lane & 15);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int col = (rw * 4 + n) * 16 + 4 * (lane >> 4);  // of 256
-          *reinterpret_cast<uint2*>(tile + m * 512 + (((col >> 3) ^ (m & 7)) << 4) + (col & 4) * 2) =
-              make_uint2(bf16_pair(acc[n][c][0], acc[n][c][1]), bf16_pair(acc[n][c][2], acc[n][c][3]));
-        }
-      }
+    for (int n = 0; n < 4; ++n) {
+      const int col = (rw * 4 + n) * 16 + 4 * (lane >> 4);  // of 256
+      *reinterpret_cast<uint2*>(tile + m * 512 + (((col >> 3) ^ (m & 7)) << 4) + (col & 4) * 2) =
+          make_uint2(bf16_pair(acc[n][c][0], acc[n][c][1]), bf16_pair(acc[n][c][2], acc[n][c][3]));
     }
-    __syncthreads();
-    for (int i = tid; i < HALF * 32; i += TILE_THREADS) {
-      const int m = i >> 5, q = i & 31, t = t0 + half * HALF + m, n = n0 + q * 8;
-      if (t >= T || n >= N) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + m * 512 + ((q ^ (m & 7)) << 4));
-      uint16_t* dst = out + (size_t)t * N + n;
-      if ((N & 7) == 0) {
-        *reinterpret_cast<u32x4*>(dst) = v;
-      } else {
+  }
+  __syncthreads();
+  for (int i = tid; i < M * 32; i += TILE_THREADS) {
+    const int m = i >> 5, q = i & 31, t = t0 + m, n = n0 + q * 8;
+    if (t >= T || n >= N) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(tile + m * 512 + ((q ^ (m & 7)) << 4));
+    uint16_t* dst = out + (size_t)t * N + n;
+    if ((N & 7) == 0) {
+      *reinterpret_cast<u32x4*>(dst) = v;
+    } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (n + k < N) dst[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
-      }
+      for (int k = 0; k < 8; ++k)
+        if (n + k < N) dst[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
     }
   }
 }
@@ -894,16 +888,16 @@ __device__ __forceinline__ void by_frags(int rows, F&& f) {
   f(std::integral_constant<int, N>{});
 }
 
-// GEMM1 and SwiGLU of (route tile, NP pairs of 16 gate and 16 up rows): rows
+// GEMM1 and SwiGLU of (route tile, 16 gate and 16 up rows): rows
 // [0, I) of W13 multiply, SiLU takes rows [I, 2 I).  Workgroups past the last
 // tile end at once.  Bound by the weights' stream where most experts have routes (32 of
 // them, T = 32: whole call 111 us for 749 MB of weights, 6.7 TB/s), and where few do by
 // the activations' from the L2, 16 routes' or 32 for every 32 weight rows.
-template <int NP, int MAXFR>
+template <int MAXFR>
 __global__ void __launch_bounds__(512)
 experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
   extern __shared__ v4f s_part[];
-  const int slices = a.I / 16 / NP;
+  const int slices = a.I / 16;
   const int j = blockIdx.x % slices, n_tiles = *r.n_tiles;
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -913,11 +907,10 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
     const int4 tile = uniform(r.tiles[i]);
     by_frags<MAXFR>(tile.z, [&](auto frc) __attribute__((always_inline)) {
       constexpr int FR = decltype(frc)::value;
-      Stream<2 * NP, FR> st;
+      Stream<2, FR> st;
 #pragma unroll
-      for (int n = 0; n < 2 * NP; ++n) {
-        const int row = j * NP + (n < NP ? n : a.I / 16 + n - NP);
-        st.w[n] = a.w13 + ((size_t)tile.x * tiles + row) * KC * W4_CHUNK_BYTES + lane * 16;
+      for (int n = 0; n < 2; ++n) {
+        st.w[n] = a.w13 + ((size_t)tile.x * tiles + j + n * slices) * KC * W4_CHUNK_BYTES + lane * 16;
       }
 #pragma unroll
       for (int f = 0; f < FR; ++f) {
@@ -927,10 +920,10 @@ experts_gemm1_kernel(ExpertsW4 a, Routes r, float* __restrict__ Cf) {
       }
       st.xs_stride = a.T;
       st.run(chunk_begin(KC, wave, waves), chunk_begin(KC, wave + 1, waves), KB);
-      st.template reduce<2>(s_part, wave, waves, [&](int p, int f, const v4f* y) {
+      st.template reduce<2>(s_part, wave, waves, [&](int, int f, const v4f* y) {
         const int m = 16 * f + (lane & 15);
         if (m >= tile.z) return;
-        *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + (j * NP + p) * 16 + 4 * (lane >> 4)) =
+        *reinterpret_cast<float4*>(Cf + (size_t)(tile.y + m) * a.I + j * 16 + 4 * (lane >> 4)) =
             swiglu(y[0], y[1]);
       });
     });
@@ -1146,7 +1139,7 @@ few_gemm2_kernel(ExpertsW4 a, const float* __restrict__ Cf) {
   }
 }
 
-// The experts' products in tiles (launched with route tiles of TILE_MAX_M).  f(NC) for
+// The experts' products in tiles (route tiles of at most TILE_MAX_M).  f(NC) for
 // the fewest fragments that hold `rows`.
 template <int NC = 1, class F>
 __device__ __forceinline__ void by_rows(int rows, F&& f) {
@@ -1169,7 +1162,7 @@ __device__ __forceinline__ int4 expert_item(const Routes& r, int item, int nblk,
 // 32 of 256 experts, T = 4001: 164 us, 1.4 PFLOP/s; GEMM2 106 us, 1.1 with its fp32 rows.
 // T = 64 on six experts: 28 us for 94 MB, which 96 workgroups' loads bound (a CU streams
 // 35 to 65 GB/s, however far ahead it loads).
-__global__ void __launch_bounds__(TILE_THREADS, 2)
+__global__ void __launch_bounds__(TILE_THREADS, TILE_WGS)
 experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__ Cq, float* __restrict__ Cs) {
   __shared__ __align__(16) TileLds s;
   const int IB = a.I / BLK;
@@ -1178,7 +1171,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
   int nb;
   const int4 tile = expert_item(r, item, IB, nb);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(a.H), tiles = 2 * a.I / 16;
   const uint8_t* w[4];
 #pragma unroll
@@ -1206,13 +1199,13 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
         }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (g == 0) s.amax[rw][(cw * NC + c) * 16 + lane] = mx;
+      if (g == 0) s.amax[rw][c * 16 + lane] = mx;
     }
     __syncthreads();
     uint8_t* codes = s.x[0];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = (cw * NC + c) * 16 + (lane & 15);
+      const int m = c * 16 + (lane & 15);
       float qs, qy;
       const float sc = block_scale(fmaxf(fmaxf(s.amax[0][m], s.amax[1][m]), fmaxf(s.amax[2][m], s.amax[3][m])), qs, qy);
 #pragma unroll
@@ -1229,7 +1222,7 @@ experts_gemm1_tile_kernel(ExpertsW4 a, Routes r, int base, uint8_t* __restrict__
 }
 
 // GEMM2 of (route tile, 256 columns of the output; the last block may have 128).
-__global__ void __launch_bounds__(TILE_THREADS, 2)
+__global__ void __launch_bounds__(TILE_THREADS, TILE_WGS)
 experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __restrict__ Cq,
                           const float* __restrict__ Cs, float* __restrict__ Y) {
   __shared__ __align__(16) TileLds s;
@@ -1239,7 +1232,7 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
   int nb;
   const int4 tile = expert_item(r, item, blocks, nb);
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rw = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), cw = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KC = w4_chunks(a.I);
   const uint8_t* w[4];
 #pragma unroll
@@ -1255,7 +1248,7 @@ experts_gemm2_tile_kernel(ExpertsW4 a, Routes r, int base, const uint8_t* __rest
     tile_product<NC>(s, w, a.I, Cq, Cs, KB, 1, [&](int m) { return tile.y + min(m, tile.z - 1); }, acc);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int m = (cw * NC + c) * 16 + (lane & 15);
+      const int m = c * 16 + (lane & 15);
       if (m >= tile.z) continue;
       const int token = s.token[m];
       const float weight = s.weight[m];
@@ -1398,7 +1391,7 @@ hipError_t launch_linear_w4(const uint8_t* x, const float* xs, const uint8_t* pa
         kernel<<<grid, TILE_THREADS, 0, stream>>>(x, xs, packed, T, N, K, base, out);
       });
     };
-    switch (linear_tile_nc(T, tiles, device_cus() * (2 / TILE_CW))) {
+    switch (linear_tile_nc(T, tiles, device_cus() * TILE_WGS)) {
       case 1: tile(linear_w4_tile_kernel<1>, 1); break;
       case 2: tile(linear_w4_tile_kernel<2>, 2); break;
       case 3: tile(linear_w4_tile_kernel<3>, 3); break;
@@ -1453,7 +1446,7 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   const bool tile = experts_in_tiles(a);
   const int fr = a.T <= 16 ? 1 : 2;
   const TilePlan plan = {tile ? 0 : 16 * fr, a.I / BLK, a.H / BLK, (a.H / 16 + 15) / 16, a.I / BLK,
-                         1.0f / (float)(device_cus() * (2 / TILE_CW))};
+                         1.0f / (float)(device_cus() * TILE_WGS)};
   if (picks <= SORT_SMALL) {
     sort_small_kernel<<<2, SORT_THREADS, 0, stream>>>(a.ids, a.weights, picks, a.k, a.e_local, a.offset, plan, r);
   } else {
@@ -1486,8 +1479,8 @@ hipError_t launch_experts_w4(const ExpertsW4& a, uint8_t* ws, hipStream_t stream
   {
     const int w = waves_of(a.H);
     const unsigned grid = grid_of(a.I / 16);
-    if (fr == 1) experts_gemm1_kernel<1, 1><<<grid, 64 * w, w * 2 * 1024, stream>>>(a, r, Cf);
-    else experts_gemm1_kernel<1, 2><<<grid, 64 * w, w * 4 * 1024, stream>>>(a, r, Cf);
+    if (fr == 1) experts_gemm1_kernel<1><<<grid, 64 * w, w * 2 * 1024, stream>>>(a, r, Cf);
+    else experts_gemm1_kernel<2><<<grid, 64 * w, w * 4 * 1024, stream>>>(a, r, Cf);
     if ((err = hipGetLastError()) != hipSuccess) return err;
   }
   const size_t units = (size_t)picks * (a.I / BLK);
