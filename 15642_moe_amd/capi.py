@@ -30,7 +30,7 @@ FORWARD_EVENTS = 6
 # Operators beside the forward: enum moe_dtype, enum moe_scoring and their limits.
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = range(3)
 SCORING = {"sigmoid": 0, "softmax": 1}
-MAX_EXPERTS, MAX_TOP_K, MAX_W4_DIM = 1024, 64, 262144
+MAX_EXPERTS, MAX_TOP_K, MAX_ROUTE_T, MAX_W4_DIM = 1024, 64, 1 << 24, 262144
 
 _c_int, _c_size, _c_float, _c_vp, _c_u64 = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
 

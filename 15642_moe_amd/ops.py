@@ -308,6 +308,8 @@ def _check_router(logits, top_k, scoring):
     score = capi.SCORING.get(scoring)
     if score is None:
         raise RuntimeError(f"scoring must be one of {sorted(capi.SCORING)}, got {scoring!r}")
+    if T > capi.MAX_ROUTE_T:
+        raise RuntimeError(f"T must be <= {capi.MAX_ROUTE_T}, got {T}")
     if not 1 <= E <= capi.MAX_EXPERTS:
         raise RuntimeError(f"logits must have 1 to {capi.MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(capi.MAX_TOP_K, E):
@@ -317,6 +319,10 @@ def _check_router(logits, top_k, scoring):
 
 def _route_topk(logits, bias, top_k, scoring, n_group, topk_group, group_top, renormalize, scale):
     T, E, stride, dtype, i, score = _check_router(logits, top_k, scoring)
+    # here, where numbers past 32 bits are still what they are
+    if not 1 <= topk_group <= n_group <= 64 or not 1 <= group_top <= 2:
+        raise RuntimeError(f"n_group must be in [1, 64], topk_group in [1, n_group], group_top 1 or 2, got {n_group}, "
+                           f"{topk_group}, {group_top}")
     dev = logits.device
     if bias is not None:
         if bias.dtype != _F32 or bias.shape != (E,) or not bias.is_contiguous():
@@ -546,6 +552,8 @@ def experts_w4(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w2: to
     _on("weights", weights, x, i)
     if weights.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("experts_w4 has no gradient: call it under torch.no_grad(), or with weights.detach()")
+    if not 0 <= local_offset <= 1 << 30:
+        raise RuntimeError(f"local_expert_offset must be in [0, 2^30], got {local_offset}")
     k, dev = ids.size(1), x.device
     ws_bytes = _experts_w4_workspace(T, K, inter, E, k)
     out = _empty(T, K, _BF16, dev)

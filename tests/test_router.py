@@ -403,3 +403,14 @@ def test_route_topk_captured_training_step(ops, cuda, scoring):
         torch.cuda.synchronize()
         for a, b in zip(captured, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_route_topk_refuses_numbers_past_32_bits(ops, cuda):
+    x = torch.zeros(2, 64, device=cuda)
+    for kw in ({"n_group": (1 << 32) + 1}, {"n_group": 8, "topk_group": (1 << 32) + 2}, {"n_group": 8, "group_top": (1 << 32) + 1},
+               {"topk_group": -1}):
+        with pytest.raises(RuntimeError, match="n_group"):
+            ops.route_topk(x, None, 2, **kw)
+    with pytest.raises(RuntimeError, match="T must be"):
+        ops.route_topk(x[:1].expand((1 << 32) + 2, 64), None, 2)

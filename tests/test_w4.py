@@ -734,3 +734,13 @@ def test_w4_two_graphs(ops, cuda):
         torch.cuda.synchronize()
         for _, out, want, _ in runs:
             assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_experts_w4_refuses_offsets_past_32_bits(ops, cuda):
+    x, s = torch.zeros(1, 128, dtype=torch.uint8, device=cuda).view(F8), torch.zeros(1, 1, device=cuda)
+    w13, w2 = (torch.zeros(1, n, 1, 4352, dtype=torch.uint8, device=cuda) for n in (16, 8))
+    ids, weights = torch.zeros(1, 1, dtype=torch.int32, device=cuda), torch.ones(1, 1, device=cuda)
+    for offset in (-1, 1 << 32, (1 << 30) + 1):
+        with pytest.raises(RuntimeError, match="local_expert_offset"):
+            ops.experts_w4(x, s, w13, w2, ids, weights, offset)
